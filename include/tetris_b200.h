@@ -324,6 +324,94 @@ int tetris_filter_load(const char *path, int device, tetris_filter_t **out);
 int tetris_filter_file_check(const char *path, tetris_filter_info_t *info);
 
 /*
+ * 4-bit filters and products (microscaled 4-bit floating point).  No counterpart in the reference.
+ * A 1x1 layer on NHWC activations is a matrix product Y[row][oc] = sum_ic X[row][ic] W[oc][ic], a
+ * row being a pixel; so is a fully connected layer.  These calls hold X and W in 4 bits with a scale
+ * per block of a row and multiply them on the tensor cores, sums in FP32.
+ *
+ * Codes are E2M1: bit 3 the sign, bits 0-2 a magnitude out of {0, 0.5, 1, 1.5, 2, 3, 4, 6}.
+ *   TETRIS_FP4_MX  blocks of 32 columns; scale 2^e as a byte e + 127 (E8M0),
+ *                  e = floor(log2(largest |x|)) - 2, at least -127; `exponent` has to be 0
+ *   TETRIS_FP4_NV  blocks of 16 columns of u = x * 2^-exponent; scale = (largest |u|) / 6 rounded
+ *                  to E4M3 (at most 448).  2688 * 2^exponent is the largest value that can be held,
+ *                  blocks whose largest value is at most 6 * 2^(exponent - 10) become zero.
+ *                  The tensor's own scale is a power of two so that every border between two codes
+ *                  is an exact FP32 number: quantisation is exact, not off by a rounding now and then.
+ * A code is x (u) over its block's scale, rounded to nearest, ties to the even code, at most 6.  A block with an infinity or a NaN takes the scale NaN (0xFF; 0x7F) and reads back
+ * as NaN, as does every product through it.  -100 <= exponent <= 100.
+ * Sums run in FP32; results below FP32's normal numbers may become zero.
+ *
+ * Storage of a matrix of `rows` x `cols`, the columns being what a product sums over:
+ *   codes   a row is `pitch` bytes, pitch = ceil(cols / 32) * 16, the even column in the low half of
+ *           a byte, zeros behind the last column
+ *   scales  tiles of 512 bytes = 128 rows x 4 blocks, as the tensor core reads them: block 4 t + j of
+ *           row r is byte (r % 32) * 16 + (r / 32 % 4) * 4 + j of tile (r / 128) * T + t, where
+ *           T = ceil(cols / 128) (MX) or ceil(cols / 64) (NV).  Zeros behind a row's last block; the
+ *           bytes of rows past the last one are neither written nor read as scales.
+ * Both 16-byte aligned.  tetris_fp4_sizes gives the bytes.
+ *
+ * Types of activations, results and dense weights: TETRIS_FP32, TETRIS_BF16, TETRIS_FP16; `ld` is the
+ * distance between rows in elements (0: rows lie close).  Tensors need the alignment of their type only;
+ * 16-byte aligned rows take the vector paths.  An output must not overlap an input.
+ * The calls are asynchronous on `stream`, allocate nothing and keep nothing between calls; the device
+ * of the filter is made current for the call, the calls without a filter run on the current device.
+ * Results are bit-reproducible from call to call.
+ */
+enum { TETRIS_FP4_MX = 0, TETRIS_FP4_NV = 1 };
+enum { TETRIS_FP32 = 0, TETRIS_BF16 = 1, TETRIS_FP16 = 2 };
+#define TETRIS_FP4_EXPONENT_AUTO 0x7FFFFFFF /* filters: the smallest exponent that holds the largest weight */
+
+int tetris_fp4_sizes(int64_t rows, int cols, int format, int64_t *pitch, int64_t *code_bytes, int64_t *scale_bytes);
+int tetris_fp4_quantize(const void *d_x, int x_type, int64_t rows, int cols, int64_t ld, int format, int exponent,
+                        void *d_codes, void *d_scales, void *stream);
+int tetris_fp4_dequantize(const void *d_codes, const void *d_scales, int64_t rows, int cols, int format, int exponent,
+                          void *d_y, int y_type, int64_t ld, void *stream);
+
+/*
+ * A 4-bit filter: the weights of a 1x1 layer (kernel_size must be 1), dense [out_channel][in_channel],
+ * borrowed, in host memory or on `device` (there complete in the order of `stream`).  Quantised on the
+ * device; the call returns when the filter is ready.
+ *   tetris_fp4_filter_download  codes (out_channel * pitch bytes) and scales as stored, either may be NULL
+ *   tetris_fp4_filter_check     waits for the device; TETRIS_ERR_CUDA if a product of this filter gave up
+ *                               on one of its bounded barrier waits since the last check (its output is
+ *                               invalid)
+ */
+typedef struct tetris_fp4_filter tetris_fp4_filter_t; /* opaque; owns device buffers */
+typedef struct {
+  int in_channel, out_channel;
+  int format, exponent;
+  int64_t pitch, code_bytes, scale_bytes;
+  int device;
+  int reserved[5];
+} tetris_fp4_filter_info_t;
+int tetris_fp4_filter_create(const void *weights, int w_type, int in_channel, int out_channel, int kernel_size,
+                             int format, int exponent, int device, void *stream, tetris_fp4_filter_t **out);
+void tetris_fp4_filter_destroy(tetris_fp4_filter_t *f);
+int tetris_fp4_filter_info(const tetris_fp4_filter_t *f, tetris_fp4_filter_info_t *info);
+int tetris_fp4_filter_download(const tetris_fp4_filter_t *f, void *codes, void *scales);
+int tetris_fp4_filter_check(const tetris_fp4_filter_t *f);
+
+/*
+ * Products with a filter; y[row][oc], bias (FP32, out_channel values) may be NULL, flags: TETRIS_FUSE_RELU.
+ *   tetris_fp4_product  activations that are quantised already, in the filter's format
+ *   tetris_fp4_linear   floating-point activations, quantised on the way (the same result as
+ *                       tetris_fp4_quantize and tetris_fp4_product)
+ *   tetris_fp4_conv2d   the 1x1 layer: FP32 NHWC in and out as tetris_conv2d_launch, padding must be 0
+ * `d_workspace` holds the quantised activations: tetris_fp4_workspace(f, rows) bytes (rows = N * OH * OW
+ * for the layer), 16-byte aligned, NULL where that is 0; free again when the call has passed on
+ * its stream.
+ */
+int tetris_fp4_product(const tetris_fp4_filter_t *f, const void *d_codes, const void *d_scales, int64_t rows, int exponent,
+                       const float *d_bias, void *d_y, int y_type, int64_t ld, int flags, void *stream);
+int tetris_fp4_workspace(const tetris_fp4_filter_t *f, int64_t rows, int64_t *bytes);
+int tetris_fp4_linear(const tetris_fp4_filter_t *f, const void *d_x, int x_type, int64_t rows, int64_t ld_x, int exponent,
+                      const float *d_bias, void *d_y, int y_type, int64_t ld_y, int flags, void *d_workspace,
+                      int64_t workspace_bytes, void *stream);
+int tetris_fp4_conv2d(const tetris_fp4_filter_t *f, const float *d_input_nhwc, float *d_output_nhwc, int batch_size,
+                      int img_h, int img_w, int stride, int padding, int exponent, const float *d_bias, int flags,
+                      void *d_workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Number of convolution kernels the library has launched in this process so far (every variant,
  * every device and thread; tuning launches included).  No counterpart in the reference; lets a
  * harness check that a timing loop really issued warm + repeat launches.

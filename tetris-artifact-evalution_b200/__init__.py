@@ -54,9 +54,17 @@ class FilterInfo(ctypes.Structure):
     ]
 
 
+class Fp4FilterInfo(ctypes.Structure):
+    _fields_ = [("in_channel", ctypes.c_int), ("out_channel", ctypes.c_int), ("format", ctypes.c_int),
+                ("exponent", ctypes.c_int), ("pitch", ctypes.c_int64), ("code_bytes", ctypes.c_int64),
+                ("scale_bytes", ctypes.c_int64), ("device", ctypes.c_int), ("reserved", ctypes.c_int * 5)]
+
+
 # name -> (restype, argtypes); the list must match include/tetris_b200.h
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
+_c_int64_p = ctypes.POINTER(ctypes.c_int64)
 SIGNATURES = {
     "tetris_filter_create": (_I, [_VP, _I, _I, _I, _I, _I, ctypes.POINTER(_VP)]),
     "tetris_filter_create_ex": (_I, [_VP, _I, _I, _I, _I, _I, ctypes.POINTER(FilterOpts), ctypes.POINTER(_VP)]),
@@ -91,6 +99,18 @@ SIGNATURES = {
     "tetris_filter_save": (_I, [_VP, ctypes.c_char_p]),
     "tetris_filter_load": (_I, [ctypes.c_char_p, _I, ctypes.POINTER(_VP)]),
     "tetris_filter_file_check": (_I, [ctypes.c_char_p, ctypes.POINTER(FilterInfo)]),
+    "tetris_fp4_sizes": (_I, [_L, _I, _I, _c_int64_p, _c_int64_p, _c_int64_p]),
+    "tetris_fp4_quantize": (_I, [_VP, _I, _L, _I, _L, _I, _I, _VP, _VP, _VP]),
+    "tetris_fp4_dequantize": (_I, [_VP, _VP, _L, _I, _I, _I, _VP, _I, _L, _VP]),
+    "tetris_fp4_filter_create": (_I, [_VP, _I, _I, _I, _I, _I, _I, _I, _VP, ctypes.POINTER(_VP)]),
+    "tetris_fp4_filter_destroy": (None, [_VP]),
+    "tetris_fp4_filter_info": (_I, [_VP, ctypes.POINTER(Fp4FilterInfo)]),
+    "tetris_fp4_filter_download": (_I, [_VP, _VP, _VP]),
+    "tetris_fp4_filter_check": (_I, [_VP]),
+    "tetris_fp4_product": (_I, [_VP, _VP, _VP, _L, _I, _VP, _VP, _I, _L, _I, _VP]),
+    "tetris_fp4_workspace": (_I, [_VP, _L, _c_int64_p]),
+    "tetris_fp4_linear": (_I, [_VP, _VP, _I, _L, _L, _I, _VP, _VP, _I, _L, _I, _VP, _L, _VP]),
+    "tetris_fp4_conv2d": (_I, [_VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _I, _VP, _L, _VP]),
     "tetris_launch_count": (ctypes.c_ulonglong, []),
     "tetris_test_inject": (ctypes.c_int, [ctypes.c_int, ctypes.c_uint]),
     "tetris_last_error": (ctypes.c_char_p, []),
@@ -410,6 +430,222 @@ def nchw_to_nhwc(src, dst, N, C, H, W, cuda_stream=None):
 
 def nhwc_to_nchw(src, dst, N, C, H, W, cuda_stream=None):
     _check(lib().tetris_nhwc_to_nchw(_ptr(src), _ptr(dst), N, C, H, W, _stream_ptr(cuda_stream)))
+
+
+# ---- 4-bit filters and products --------------------------------------------------------------
+FP4_MX, FP4_NV = 0, 1             # blocks of 32 with power-of-two scales; blocks of 16 with E4M3 scales
+FP32, BF16, FP16 = 0, 1, 2        # types of activations and results
+FP4_EXPONENT_AUTO = 0x7FFFFFFF    # filters: the smallest exponent that holds the largest weight
+
+_FP4_TYPES = {"torch.float32": FP32, "torch.bfloat16": BF16, "torch.float16": FP16}
+_fp4_type_of = {}                 # torch dtype -> type, filled as dtypes are met
+
+
+def _fp4_type(x, dtype, what):
+    """The type of a dense argument: `dtype` for an address, the tensor's own for a tensor."""
+    if isinstance(x, int):
+        return FP32 if dtype is None else dtype
+    t = _fp4_type_of.get(x.dtype)
+    if t is None:
+        t = _FP4_TYPES.get(str(x.dtype))
+        if t is None:
+            raise ValueError("%s of type %s: FP32, BF16 or FP16 are covered" % (what, x.dtype))
+        _fp4_type_of[x.dtype] = t
+    if dtype is not None and dtype != t:
+        raise ValueError("%s is a tensor of type %s, another type was named" % (what, x.dtype))
+    return t
+
+
+def _fp4_dense(x, rows, cols, ld, what):
+    """(address, row distance) of a dense device matrix of rows x cols.  A two-dimensional tensor may have
+    rows further apart than cols; any other has to be contiguous."""
+    if isinstance(x, int):
+        return x, ld
+    if x.dim() == 2 and x.shape[0] == rows and x.shape[1] == cols:
+        if rows > 1 or cols > 1:
+            apart, step = x.stride()
+            if (step != 1 and cols > 1) or (apart < cols and rows > 1):
+                raise ValueError("the columns of %s have to lie side by side, its strides are %s" % (what, tuple(x.stride())))
+            if ld and rows > 1 and ld != apart:
+                raise ValueError("rows of %s lie %d elements apart, %d was named" % (what, apart, ld))
+            if rows > 1:
+                return x.data_ptr(), apart
+        return x.data_ptr(), 0
+    if not x.is_contiguous():
+        raise ValueError("%s is neither a %d x %d matrix nor contiguous" % (what, rows, cols))
+    need = (rows - 1) * (ld or cols) + cols if rows else 0
+    if x.numel() < need:
+        raise ValueError("%s has %d elements, %d are needed" % (what, x.numel(), need))
+    return x.data_ptr(), ld
+
+
+def _fp4_bytes(x, need, what):
+    """Address of a device buffer of at least `need` bytes."""
+    if isinstance(x, int):
+        return x
+    if not x.is_contiguous() or x.numel() * x.element_size() < need:
+        raise ValueError("%s has to be contiguous and hold %d bytes" % (what, need))
+    return x.data_ptr()
+
+
+def _fp4_bias(bias, out_channel):
+    if bias is None or isinstance(bias, int):
+        return bias
+    if _fp4_type(bias, None, "bias") != FP32 or not bias.is_contiguous() or bias.numel() < out_channel:
+        raise ValueError("the bias has to be %d contiguous float32 values" % out_channel)
+    return bias.data_ptr()
+
+
+def _fp4_storage(rows, cols, format):
+    """(code bytes, scale bytes) as tetris_fp4_sizes computes them."""
+    block = 16 if format == FP4_NV else 32
+    return rows * ((cols + 31) // 32 * 16), (rows + 127) // 128 * ((cols + 4 * block - 1) // (4 * block)) * 512
+
+
+def fp4_sizes(rows, cols, format):
+    """(bytes of the codes, bytes of the scales) of a rows x cols matrix in 4 bits."""
+    c, s = ctypes.c_int64(0), ctypes.c_int64(0)
+    _check(lib().tetris_fp4_sizes(rows, cols, format, None, ctypes.byref(c), ctypes.byref(s)))
+    return c.value, s.value
+
+
+def fp4_quantize(input, codes, scales, rows, cols, format, exponent=0, ld=0, dtype=None, cuda_stream=None):
+    """Device `input` (rows x cols, FP32 / BF16 / FP16) -> `codes` and `scales` (uint8 device buffers of
+    fp4_sizes bytes), asynchronous.  `exponent`: of the whole tensor, FP4_NV only."""
+    need = _fp4_storage(rows, cols, format)
+    x, ld = _fp4_dense(input, rows, cols, ld, "the input")
+    _check(lib().tetris_fp4_quantize(x, _fp4_type(input, dtype, "the input"), rows, cols, ld, format, exponent,
+                                     _fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"),
+                                     _stream_ptr(cuda_stream)))
+
+
+def fp4_dequantize(codes, scales, output, rows, cols, format, exponent=0, ld=0, dtype=None, cuda_stream=None):
+    """The values that `codes` and `scales` stand for, into device `output` (rows x cols), asynchronous."""
+    need = _fp4_storage(rows, cols, format)
+    y, ld = _fp4_dense(output, rows, cols, ld, "the output")
+    _check(lib().tetris_fp4_dequantize(_fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"), rows, cols,
+                                       format, exponent, y, _fp4_type(output, dtype, "the output"), ld, _stream_ptr(cuda_stream)))
+
+
+class Fp4Filter:
+    """The weights of a 1x1 (or fully connected) layer in 4 bits, living on one GPU.
+
+    Beside SparseFilter: dense [out_channel][in_channel] `filter` (numpy array, or a tensor on the host
+    or on `device`), quantised on the device.  `exponent` is the whole filter's in the FP4_NV format
+    (FP4_EXPONENT_AUTO: the smallest that holds the largest weight).  It owns device memory, freed by
+    close() or garbage collection.
+    """
+
+    def __init__(self, filter, in_channel, out_channel, kernel_size=1, format=FP4_MX, exponent=FP4_EXPONENT_AUTO, device=None,
+                 cuda_stream=None):
+        self._handle = _VP()
+        if hasattr(filter, "data_ptr"):
+            if not filter.is_contiguous():
+                raise ValueError("the filter has to be contiguous")
+            if device is None:
+                device = filter.device.index if filter.is_cuda else 0
+            size, kind, address = filter.numel(), _fp4_type(filter, None, "the filter"), filter.data_ptr()
+        else:
+            filter = np.ascontiguousarray(filter, dtype=np.float32)
+            size, kind, address = filter.size, FP32, filter.ctypes.data
+        if size != in_channel * out_channel * kernel_size * kernel_size:
+            raise ValueError("filter has %d elements, expected %d" % (size, in_channel * out_channel * kernel_size * kernel_size))
+        _check(lib().tetris_fp4_filter_create(address, kind, in_channel, out_channel, kernel_size, format, exponent, device or 0,
+                                              _stream_ptr(cuda_stream), ctypes.byref(self._handle)))
+        info = self.info()
+        self.in_channel_, self.out_channel_ = info.in_channel, info.out_channel
+        self.format_, self.exponent_, self.device_ = info.format, info.exponent, info.device
+
+    def info(self):
+        info = Fp4FilterInfo()
+        _check(lib().tetris_fp4_filter_info(self.handle, ctypes.byref(info)))
+        return info
+
+    def download(self):
+        """(codes uint8[out_channel, pitch], scales uint8[bytes]) copied back from the device."""
+        info = self.info()
+        codes = np.empty((info.out_channel, info.pitch), np.uint8)
+        scales = np.empty(info.scale_bytes, np.uint8)
+        _check(lib().tetris_fp4_filter_download(self._handle, codes.ctypes.data, scales.ctypes.data))
+        return codes, scales
+
+    def check(self):
+        """Synchronise and raise if a product of this filter timed out on a barrier."""
+        _check(lib().tetris_fp4_filter_check(self.handle))
+
+    @property
+    def handle(self):
+        if not self._handle:
+            raise RuntimeError("Fp4Filter already closed")
+        return self._handle
+
+    def close(self):
+        if getattr(self, "_handle", None):
+            lib().tetris_fp4_filter_destroy(self._handle)
+            self._handle = _VP()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def fp4_product(fp4_filter, codes, scales, output, rows, exponent=0, bias=None, relu=False, ld=0, dtype=None, cuda_stream=None):
+    """`output` (device, rows x out_channel) = quantised activations times the filter (+ bias, ReLU),
+    asynchronous; `codes` and `scales` as fp4_quantize writes them in the filter's format."""
+    f = fp4_filter
+    need = _fp4_storage(rows, f.in_channel_, f.format_)
+    y, ld = _fp4_dense(output, rows, f.out_channel_, ld, "the output")
+    _check(lib().tetris_fp4_product(f.handle, _fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"), rows,
+                                    exponent, _fp4_bias(bias, f.out_channel_), y, _fp4_type(output, dtype, "the output"), ld,
+                                    FUSE_RELU if relu else 0, _stream_ptr(cuda_stream)))
+
+
+def fp4_workspace(fp4_filter, rows):
+    """Bytes of device workspace that fp4_linear and fp4_conv2d need for `rows` rows (pixels)."""
+    n = ctypes.c_int64(0)
+    _check(lib().tetris_fp4_workspace(fp4_filter.handle, rows, ctypes.byref(n)))
+    return n.value
+
+
+def _fp4_room(workspace):
+    """(address, bytes) of a workspace; an address is taken to be large enough."""
+    if workspace is None:
+        return None, 0
+    if isinstance(workspace, int):
+        return workspace, 1 << 62
+    if not workspace.is_contiguous():
+        raise ValueError("the workspace has to be contiguous")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def fp4_linear(fp4_filter, input, output, rows, workspace=None, exponent=0, bias=None, relu=False, ld_input=0, ld_output=0,
+               input_dtype=None, output_dtype=None, cuda_stream=None):
+    """`output` (rows x out_channel) = `input` (rows x in_channel, FP32 / BF16 / FP16), quantised on the way,
+    times the filter (+ bias, ReLU), asynchronous.  `workspace`: fp4_workspace bytes on the device."""
+    f = fp4_filter
+    x, ld_input = _fp4_dense(input, rows, f.in_channel_, ld_input, "the input")
+    y, ld_output = _fp4_dense(output, rows, f.out_channel_, ld_output, "the output")
+    room = _fp4_room(workspace)
+    _check(lib().tetris_fp4_linear(f.handle, x, _fp4_type(input, input_dtype, "the input"), rows, ld_input, exponent,
+                                   _fp4_bias(bias, f.out_channel_), y, _fp4_type(output, output_dtype, "the output"), ld_output,
+                                   FUSE_RELU if relu else 0, room[0], room[1], _stream_ptr(cuda_stream)))
+
+
+def fp4_conv2d(fp4_filter, input, output, batch_size, img_h, img_w, stride, padding, workspace=None, exponent=0, bias=None,
+               relu=False, cuda_stream=None):
+    """The 1x1 layer with a 4-bit filter: device NHWC FP32 in and out as sparse_conv2d, padding 0."""
+    f = fp4_filter
+    pixels = batch_size * ((img_h - 1) // stride + 1) * ((img_w - 1) // stride + 1) if stride > 0 else 0
+    if _fp4_type(input, None, "the input") != FP32 or _fp4_type(output, None, "the output") != FP32:
+        raise ValueError("a 4-bit layer takes and gives float32")
+    x = _fp4_bytes(input, 4 * batch_size * img_h * img_w * f.in_channel_, "the input")
+    y = _fp4_bytes(output, 4 * pixels * f.out_channel_, "the output")
+    room = _fp4_room(workspace)
+    _check(lib().tetris_fp4_conv2d(f.handle, x, y, batch_size, img_h, img_w, stride, padding, exponent,
+                                   _fp4_bias(bias, f.out_channel_), FUSE_RELU if relu else 0, room[0], room[1],
+                                   _stream_ptr(cuda_stream)))
 
 
 def filter_file_check(path):
