@@ -3,37 +3,47 @@
 // Mathematics.  A block (32 values in the MX form, 16 in the NV form) has one scale s, a code is
 // RNE(x / s) onto {0, .5, 1, 1.5, 2, 3, 4, 6}.
 //   MX: s = 2^e with e + 127 = max(exponent field of the largest |x| - 2, 0): x / s is exact.
-//   NV: s = 2^exponent * E4M3(largest |x| / (6 * 2^exponent)).  Both roundings have to be those of the
-//       exact quotient.  The division by 6 is IEEE's: a quotient of 24 bits by 6 differs from a border
-//       of E4M3 (at most 5 bits) by 0 or by more than half of its own last place, so rounding it to 24
-//       bits first changes nothing.  The same holds for x / s, s having 4 significant bits and a border
-//       between codes 3: half a last place of the quotient is less than the distance of the nearest x
-//       that is not on the border.  That quotient is taken as q = x r with r = 1 / s rounded, corrected by
-//       the exact remainder (Markstein: q + r (x - q s), the correctly rounded quotient).
+//   NV: s = 2^exponent * E4M3(largest |x| / (6 * 2^exponent)).  Both roundings have to be those of the exact
+//       quotient.  A quotient of 24 bits by s (4 significant bits) that is not on a border between codes (3
+//       bits) lies more than half of its last place away from it, and so does one by 6 from a border of
+//       E4M3 (5 bits): rounded to 24 bits it stays on its side, and on the border it stays there, if only
+//       the error before that rounding is small.  So the quotient is x r + x r', r an approximate reciprocal
+//       and r' = r (1 - r s) its Newton correction: two operations a value (checked for every 24-bit x,
+//       every s and border).
 //
-// Bound: HBM.  A thread takes 16 bytes of a row, the threads of a block find their largest value with
-// shuffles, so that every load and store of a warp is contiguous; kChunks independent chunks per thread
-// keep loads in flight.
+// Bound: HBM; what stands in its way is the number of instructions, so a thread keeps one column position
+// and walks down kRows rows, takes 8 values at a time, and finds the largest one of 16-bit types as packed
+// integers.  4096 x 8192: see the figures at the launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "fp4.h"
 
 namespace tetris {
 namespace {
 
-constexpr int kThreads = 256, kChunks = 4;
+constexpr int kThreads = 256, kRows = 4;
+
+// How a block of threads covers a matrix cut into pieces of 8 columns: 2^lx threads side by side, the others
+// below them, and again `ROWS` times.
+struct Walk {
+  int lx;
+  uint32_t col_blocks;
+};
 
 struct QuantizeParams {
   const void *x;
   uint8_t *codes, *scales;
-  int64_t rows, ld, pitch;
-  int64_t total;           // chunks of all rows
+  uint32_t rows;
+  int64_t ld, pitch;
   int cols, tiles;         // tiles: scale tiles of a row
-  int exponent;
-  Fp4Div by_chunks;        // chunks of a row, whole scale tiles
+  Walk walk;
+  int wide;                // 32-byte aligned rows
+  float tensor_scale;      // 2^exponent
+  float sixth, sixth_rest; // 1 / (6 * 2^exponent) and what its rounding left
   Fp4Pixels px;
   Fp4Div by_OH, by_OW;
 };
@@ -46,14 +56,61 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// 8 values as they were loaded, and what is asked of them.
+template <typename T> struct Piece {  // 16-bit types
+  uint4 raw;
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const T *src, bool) { raw = *reinterpret_cast<const uint4 *>(src); }
+  __device__ __forceinline__ void set(int k, T v) {
+    const uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&v) << (16 * (k & 1));
+    (k < 2 ? raw.x : k < 4 ? raw.y : k < 6 ? raw.z : raw.w) |= b;
+  }
+  // Bits of |x|, two values side by side: as integers they are ordered like the numbers, NaN last.
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t m = 0x7FFF7FFFu;
+    return __vmaxu2(__vmaxu2(raw.x & m, raw.y & m), __vmaxu2(raw.z & m, raw.w & m));
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ float number(uint32_t t) {
+    const uint16_t b = (uint16_t)max(t & 0xFFFFu, t >> 16);
+    return to_float(*reinterpret_cast<const T *>(&b));
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = to_float(e[k]);
+  }
+};
+template <> struct Piece<float> {
+  float v[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float *src, bool wide) {
+    if (wide) {
+      asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(src));
+    } else {
+      *reinterpret_cast<float4 *>(v) = reinterpret_cast<const float4 *>(src)[0];
+      *reinterpret_cast<float4 *>(v + 4) = reinterpret_cast<const float4 *>(src)[1];
+    }
+  }
+  __device__ __forceinline__ void set(int k, float x) { v[k] = x; }
+  __device__ __forceinline__ uint32_t top() const {
+    float t = fabsf(v[0]);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t) : "f"(fabsf(v[k])));
+    return __float_as_uint(t);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ float number(uint32_t t) { return __uint_as_float(t); }
+  __device__ __forceinline__ void values(float (&w)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = v[k];
+  }
+};
 
-// max that hands a NaN on
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // codes of 8 values, the first in the lowest 4 bits (RNE, at most 6)
 __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
   uint32_t r;
@@ -63,14 +120,6 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
       "mov.b32 %0, {a, b, c, d};\n}"
       : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
-}
-__device__ __forceinline__ uint16_t codes_of(const float (&v)[4]) {
-  uint32_t r;
-  asm("{\n.reg .b8 a, b;\n"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
-      "mov.b32 %0, {a, b, a, b};\n}"
-      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
-  return (uint16_t)r;
 }
 __device__ __forceinline__ uint8_t e4m3_of(float v) {  // RNE, at most 448
   uint16_t r;
@@ -84,109 +133,99 @@ __device__ __forceinline__ float e4m3_value(uint8_t b) {
 }
 
 // The values of a thread's part of a block become quotients by the block's scale; returns the scale's byte.
-template <int FMT, int CV>
-__device__ __forceinline__ uint8_t scale_block(float (&v)[CV], float top, int exponent) {
+template <int FMT>
+__device__ __forceinline__ uint8_t scale_block(float (&v)[8], float top, float tensor_scale, float sixth, float sixth_rest) {
   if (!(top < __int_as_float(0x7F800000))) {  // codes of 1: the block is NaN whatever it meets
 #pragma unroll
-    for (int i = 0; i < CV; ++i) v[i] = 1.f;
+    for (int i = 0; i < 8; ++i) v[i] = 1.f;
     return FMT == TETRIS_FP4_NV ? 0x7F : 0xFF;
   }
   if (FMT == TETRIS_FP4_MX) {
     const int byte = max((int)(__float_as_uint(top) >> 23) - 2, 0);  // at most 252
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
 #pragma unroll
-    for (int i = 0; i < CV; ++i) v[i] *= inv;
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
     return (uint8_t)byte;
   }
-  const uint8_t byte = e4m3_of(__fdiv_rn(top * pow2f(-exponent), 6.f));
-  const float s = e4m3_value(byte) * pow2f(exponent);
+  const float within = fminf(top, 4096.f * tensor_scale);  // (beyond 2688 the scale stays at its largest)
+  const uint8_t byte = e4m3_of(__fmaf_rn(within, sixth, within * sixth_rest));
+  const float s = e4m3_value(byte) * tensor_scale;
   if (top > 1e3f * s && s > 0.f) {  // far above what the exponent holds: x / s could leave FP32
     const float most = 1e3f * s;
 #pragma unroll
-    for (int i = 0; i < CV; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
+    for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
   }
-  const float r = s > 0.f ? __frcp_rn(s) : 0.f;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  if (s == 0.f) r = 0.f;
+  const float rest = __fmaf_rn(-r, s, 1.f) * r;
 #pragma unroll
-  for (int i = 0; i < CV; ++i) {
-    const float q = v[i] * r;
-    v[i] = __fmaf_rn(__fmaf_rn(-q, s, v[i]), r, q);
-  }
+  for (int i = 0; i < 8; ++i) v[i] = __fmaf_rn(v[i], r, v[i] * rest);
   return byte;
 }
 
-__device__ __forceinline__ int64_t scale_at(int64_t row, int blk, int tiles) {
-  return ((row >> 7) * tiles + (blk >> 2)) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4 + (blk & 3);
-}
-
-template <typename T, int FMT, bool VEC, bool STRIDED>
+template <typename T, int FMT, bool VEC, bool STRIDED, int ROWS>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams p) {
-  constexpr int CV = 16 / sizeof(T);                                  // values of a chunk
   constexpr int kBlock = FMT == TETRIS_FP4_NV ? 16 : 32;
-  constexpr int kLanes = kBlock / CV;                                 // threads of a block
+  constexpr int kLanes = kBlock / 8;                                  // threads of a block of values
   grid_release();
   grid_wait();
-  float v[kChunks][CV];
-  uint32_t chunk[kChunks];
-  int64_t row[kChunks];
-  const int64_t at = (int64_t)blockIdx.x * (kThreads * kChunks) + threadIdx.x;
+  const uint32_t row_block = blockIdx.x / p.walk.col_blocks, col_block = blockIdx.x - row_block * p.walk.col_blocks;
+  const uint32_t below = kThreads >> p.walk.lx;
+  const uint32_t piece = (col_block << p.walk.lx) + (threadIdx.x & ((1u << p.walk.lx) - 1u));
+  const uint32_t row0 = row_block * (below * ROWS) + (threadIdx.x >> p.walk.lx);
+  const int col = (int)piece * 8, left = p.cols - col;                // (may lie behind the last column: zeros)
+  const T *x = static_cast<const T *>(p.x) + col;
+  Piece<T> in[ROWS];
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    const int64_t i = at + u * kThreads;
-    if (p.total < (1ll << 31)) {
-      const uint32_t r = fp4_quot((uint32_t)min(i, p.total), p.by_chunks);
-      row[u] = i < p.total ? r : p.rows;
-      chunk[u] = (uint32_t)i - r * p.by_chunks.d;
-    } else {
-      row[u] = i / p.by_chunks.d;
-      chunk[u] = (uint32_t)(i - row[u] * p.by_chunks.d);
-    }
-    const int col = (int)chunk[u] * CV;
-#pragma unroll
-    for (int k = 0; k < CV; ++k) v[u][k] = 0.f;
-    if (row[u] >= p.rows || col >= p.cols) continue;
-    int64_t from = row[u] * p.ld;
+  for (int u = 0; u < ROWS; ++u) {
+    const uint32_t row = row0 + u * below;
+    in[u].zero();
+    if (row >= p.rows || left <= 0) continue;
+    int64_t from = row;
     if (STRIDED) {
-      const uint32_t y = fp4_quot((uint32_t)row[u], p.by_OW), ox = (uint32_t)row[u] - y * p.px.OW;
+      const uint32_t y = fp4_quot(row, p.by_OW), ox = row - y * p.px.OW;
       const uint32_t n = fp4_quot(y, p.by_OH), oy = y - n * p.px.OH;
-      from = (((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S) * p.ld;
+      from = ((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S;
     }
-    const T *src = static_cast<const T *>(p.x) + from + col;
-    if (VEC && col + CV <= p.cols) {
-      const uint4 raw = *reinterpret_cast<const uint4 *>(src);
-      const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-      for (int k = 0; k < CV; ++k) v[u][k] = to_float(e[k]);
+    const T *src = x + from * p.ld;
+    if (VEC && left >= 8) {
+      in[u].load(src, p.wide);
     } else {
 #pragma unroll
-      for (int k = 0; k < CV; ++k)
-        if (col + k < p.cols) v[u][k] = to_float(src[k]);
+      for (int k = 0; k < 8; ++k)
+        if (k < left) in[u].set(k, src[k]);
     }
   }
+  const bool has_codes = col / 2 < p.pitch, has_scale = piece % kLanes == 0 && (int)(piece / (4 * kLanes)) < p.tiles;
+  const uint32_t keep = left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u;  // zeros behind the last column
+  uint8_t *codes = p.codes + col / 2;
+  uint8_t *scales = p.scales + (size_t)(piece / (4 * kLanes)) * 512 + piece / kLanes % 4;
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    float top = fabsf(v[u][0]);
+  for (int u = 0; u < ROWS; ++u) {
+    const uint32_t row = row0 + u * below;
+    uint32_t top = in[u].top();
 #pragma unroll
-    for (int k = 1; k < CV; ++k) top = max_nan(top, fabsf(v[u][k]));
-#pragma unroll
-    for (int s = 1; s < kLanes; s *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const uint8_t byte = scale_block<FMT>(v[u], top, p.exponent);
-    if (row[u] >= p.rows) continue;
-    const int col = (int)chunk[u] * CV, blk = col / kBlock, left = p.cols - col;
-    auto codes = codes_of(v[u]);
-    if (left < CV) codes = left <= 0 ? 0 : codes & ((1u << (4 * left)) - 1u);  // zeros behind the last column
-    if (col / 2 < p.pitch) *reinterpret_cast<decltype(codes) *>(p.codes + row[u] * p.pitch + col / 2) = codes;
-    if (chunk[u] % kLanes == 0) p.scales[scale_at(row[u], blk, p.tiles)] = byte;
+    for (int s = 1; s < kLanes; s *= 2) top = Piece<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, s));
+    float v[8];
+    in[u].values(v);
+    const uint8_t byte = scale_block<FMT>(v, Piece<T>::number(top), p.tensor_scale, p.sixth, p.sixth_rest);
+    const uint32_t c = codes_of(v) & keep;
+    if (row >= p.rows) continue;
+    if (has_codes) *reinterpret_cast<uint32_t *>(codes + row * p.pitch) = c;
+    if (has_scale) scales[(int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4] = byte;
   }
 }
 
 struct DequantizeParams {
   const uint8_t *codes, *scales;
   void *y;
-  int64_t rows, ld, pitch;
-  int64_t total;           // pieces of 8 columns of all rows
+  uint32_t rows;
+  int64_t ld, pitch;
   int cols, tiles;
-  int exponent;
-  Fp4Div by_pieces;
+  Walk walk;
+  int wide;                // 32-byte aligned rows
+  float tensor_scale;
 };
 
 __device__ __forceinline__ void values_of(uint32_t codes, float (&v)[8]) {
@@ -207,50 +246,60 @@ template <int FMT> __device__ __forceinline__ float scale_value(uint8_t b) {
   return b == 0xFF ? __int_as_float(0x7FC00000) : b ? __uint_as_float((uint32_t)b << 23) : __uint_as_float(0x00400000u);
 }
 
-// A thread turns 8 codes (one block's) into values.
-template <typename T, int FMT, bool VEC>
+template <typename T> __device__ __forceinline__ void store8(T *dst, const float (&v)[8], bool) {
+  alignas(16) T out[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) out[k] = from_float<T>(v[k]);
+  *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(out);
+}
+template <> __device__ __forceinline__ void store8(float *dst, const float (&v)[8], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+  } else {
+    reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+template <typename T, int FMT, bool VEC, int ROWS>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeParams p) {
-  constexpr int kBlock = FMT == TETRIS_FP4_NV ? 16 : 32;
+  constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8;
   grid_release();
   grid_wait();
-  const int64_t at = (int64_t)blockIdx.x * (kThreads * kChunks) + threadIdx.x;
-  const float tensor_scale = pow2f(p.exponent);
-  uint32_t codes[kChunks], piece[kChunks];
-  uint8_t byte[kChunks];
-  int64_t row[kChunks];
+  const uint32_t row_block = blockIdx.x / p.walk.col_blocks, col_block = blockIdx.x - row_block * p.walk.col_blocks;
+  const uint32_t below = kThreads >> p.walk.lx;
+  const uint32_t piece = (col_block << p.walk.lx) + (threadIdx.x & ((1u << p.walk.lx) - 1u));
+  const uint32_t row0 = row_block * (below * ROWS) + (threadIdx.x >> p.walk.lx);
+  const int col = (int)piece * 8, left = p.cols - col;
+  if (left <= 0) return;
+  const uint8_t *codes = p.codes + col / 2;
+  const uint8_t *scales = p.scales + (size_t)(piece / (4 * kLanes)) * 512 + piece / kLanes % 4;
+  uint32_t c[ROWS];
+  uint8_t byte[ROWS];
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    const int64_t i = at + u * kThreads;
-    if (p.total < (1ll << 31)) {
-      const uint32_t r = fp4_quot((uint32_t)min(i, p.total), p.by_pieces);
-      row[u] = i < p.total ? r : p.rows;
-      piece[u] = (uint32_t)i - r * p.by_pieces.d;
-    } else {
-      row[u] = i / p.by_pieces.d;
-      piece[u] = (uint32_t)(i - row[u] * p.by_pieces.d);
-    }
-    if (row[u] >= p.rows) continue;
-    codes[u] = *reinterpret_cast<const uint32_t *>(p.codes + row[u] * p.pitch + piece[u] * 4);
-    byte[u] = p.scales[scale_at(row[u], (int)piece[u] * 8 / kBlock, p.tiles)];
+  for (int u = 0; u < ROWS; ++u) {
+    const uint32_t row = row0 + u * below;
+    if (row >= p.rows) continue;
+    c[u] = *reinterpret_cast<const uint32_t *>(codes + row * p.pitch);
+    byte[u] = scales[(int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4];
   }
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    if (row[u] >= p.rows) continue;
+  for (int u = 0; u < ROWS; ++u) {
+    const uint32_t row = row0 + u * below;
+    if (row >= p.rows) continue;
     float v[8];
-    values_of(codes[u], v);
-    const float s = scale_value<FMT>(byte[u]) * tensor_scale;
-    const int col = (int)piece[u] * 8;
-    T *dst = static_cast<T *>(p.y) + row[u] * p.ld + col;
-    alignas(16) T out[8];
+    values_of(c[u], v);
+    const float s = scale_value<FMT>(byte[u]) * p.tensor_scale;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) out[k] = from_float<T>(v[k] * s);
-    if (VEC && col + 8 <= p.cols) {
-#pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4 *>(dst)[k] = reinterpret_cast<const uint4 *>(out)[k];
+    for (int k = 0; k < 8; ++k) v[k] *= s;
+    T *dst = static_cast<T *>(p.y) + row * p.ld + col;
+    if (VEC && left >= 8) {
+      store8(dst, v, p.wide);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (col + k < p.cols) dst[k] = out[k];
+        if (k < left) dst[k] = from_float<T>(v[k]);
     }
   }
 }
@@ -266,14 +315,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) largest_kernel
   if ((threadIdx.x & 31) == 0) atomicMax(bits, m);
 }
 
-bool vector_rows(const void *p, int64_t ld, int bytes) { return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(ld * bytes)) & 15) == 0; }
-
-int blocks_for(int64_t total, unsigned *blocks) {
-  const int64_t n = (total + kThreads * kChunks - 1) / (kThreads * kChunks);
-  if (n > 0x7FFFFFFF) { set_error("a matrix of this size is outside what the kernels cover"); return TETRIS_ERR_UNSUPPORTED; }
-  *blocks = (unsigned)n;
-  return TETRIS_OK;
-}
+bool vector_rows(const void *p, int64_t ld, int bytes, int align) { return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(ld * bytes)) & (align - 1)) == 0; }
 
 int launched(cudaError_t err) {
   if (err == cudaSuccess) return TETRIS_OK;
@@ -281,34 +323,50 @@ int launched(cudaError_t err) {
   return TETRIS_ERR_CUDA;
 }
 
-template <typename T> int quantize(QuantizeParams p, int format, bool strided, cudaStream_t st) {
-  const bool vec = vector_rows(p.x, p.ld, sizeof(T));
-  const int chunks = p.tiles * 4 * fp4_block(format) / (16 / (int)sizeof(T));
-  p.by_chunks = fp4_div((uint32_t)chunks);
-  p.total = p.rows * chunks;
-  unsigned blocks;
-  int rc = blocks_for(p.total, &blocks);
-  if (rc) return rc;
-  auto go = [&](void (*kernel)(const QuantizeParams)) { return launched(launch_overlapped(kernel, dim3(blocks), kThreads, 0, st, 1, p)); };
-  if (format == TETRIS_FP4_NV) {
-    if (strided) return vec ? go(quantize_kernel<T, TETRIS_FP4_NV, true, true>) : go(quantize_kernel<T, TETRIS_FP4_NV, false, true>);
-    return vec ? go(quantize_kernel<T, TETRIS_FP4_NV, true, false>) : go(quantize_kernel<T, TETRIS_FP4_NV, false, false>);
+// Threads side by side for `pieces` of a row: what leaves the fewest of them idle, more rather than fewer.
+// `many`: enough blocks for every SM even with kRows rows a thread (few rows are spread over more threads).
+int plan_walk(uint32_t rows, int64_t pieces, Walk *w, unsigned *blocks, bool *many) {
+  int64_t least = INT64_MAX;
+  for (int lx = 8; lx >= 2; --lx) {
+    const int64_t padded = ((pieces + (1 << lx) - 1) >> lx) << lx;
+    if (padded < least) { least = padded; w->lx = lx; }
   }
-  if (strided) return vec ? go(quantize_kernel<T, TETRIS_FP4_MX, true, true>) : go(quantize_kernel<T, TETRIS_FP4_MX, false, true>);
-  return vec ? go(quantize_kernel<T, TETRIS_FP4_MX, true, false>) : go(quantize_kernel<T, TETRIS_FP4_MX, false, false>);
+  w->col_blocks = (uint32_t)(least >> w->lx);
+  const int64_t below = kThreads >> w->lx;
+  *many = (rows + below * kRows - 1) / (below * kRows) * w->col_blocks >= 2 * 148;
+  const int64_t span = below * (*many ? kRows : 1), n = (rows + span - 1) / span * w->col_blocks;
+  if (n > 0x7FFFFFFF) { set_error("a matrix of this size is outside what the kernels cover"); return TETRIS_ERR_UNSUPPORTED; }
+  *blocks = (unsigned)n;
+  return TETRIS_OK;
 }
 
-template <typename T> int dequantize(DequantizeParams p, int format, cudaStream_t st) {
-  const bool vec = vector_rows(p.y, p.ld, sizeof(T));
-  const int pieces = (p.cols + 7) / 8;
-  p.by_pieces = fp4_div((uint32_t)pieces);
-  p.total = p.rows * pieces;
+template <typename T, int FMT, bool VEC, bool STRIDED> int quantize(const QuantizeParams &p, unsigned blocks, bool many, cudaStream_t st) {
+  return launched(many ? launch_overlapped(quantize_kernel<T, FMT, VEC, STRIDED, kRows>, dim3(blocks), kThreads, 0, st, 1, p)
+                       : launch_overlapped(quantize_kernel<T, FMT, VEC, STRIDED, 1>, dim3(blocks), kThreads, 0, st, 1, p));
+}
+template <typename T, int FMT> int quantize(QuantizeParams p, bool strided, cudaStream_t st) {
+  const bool vec = vector_rows(p.x, p.ld, sizeof(T), 16);
+  p.wide = vector_rows(p.x, p.ld, sizeof(T), 32);
   unsigned blocks;
-  int rc = blocks_for(p.total, &blocks);
+  bool many;
+  const int rc = plan_walk(p.rows, (int64_t)p.tiles * fp4_block(FMT) / 2, &p.walk, &blocks, &many);
   if (rc) return rc;
-  auto go = [&](void (*kernel)(const DequantizeParams)) { return launched(launch_overlapped(kernel, dim3(blocks), kThreads, 0, st, 1, p)); };
-  if (format == TETRIS_FP4_NV) return vec ? go(dequantize_kernel<T, TETRIS_FP4_NV, true>) : go(dequantize_kernel<T, TETRIS_FP4_NV, false>);
-  return vec ? go(dequantize_kernel<T, TETRIS_FP4_MX, true>) : go(dequantize_kernel<T, TETRIS_FP4_MX, false>);
+  if (strided) return vec ? quantize<T, FMT, true, true>(p, blocks, many, st) : quantize<T, FMT, false, true>(p, blocks, many, st);
+  return vec ? quantize<T, FMT, true, false>(p, blocks, many, st) : quantize<T, FMT, false, false>(p, blocks, many, st);
+}
+
+template <typename T, int FMT, bool VEC> int dequantize(const DequantizeParams &p, unsigned blocks, bool many, cudaStream_t st) {
+  return launched(many ? launch_overlapped(dequantize_kernel<T, FMT, VEC, kRows>, dim3(blocks), kThreads, 0, st, 1, p)
+                       : launch_overlapped(dequantize_kernel<T, FMT, VEC, 1>, dim3(blocks), kThreads, 0, st, 1, p));
+}
+template <typename T, int FMT> int dequantize(DequantizeParams p, cudaStream_t st) {
+  const bool vec = vector_rows(p.y, p.ld, sizeof(T), 16);
+  p.wide = vector_rows(p.y, p.ld, sizeof(T), 32);
+  unsigned blocks;
+  bool many;
+  const int rc = plan_walk(p.rows, ((int64_t)p.cols + 7) / 8, &p.walk, &blocks, &many);
+  if (rc) return rc;
+  return vec ? dequantize<T, FMT, true>(p, blocks, many, st) : dequantize<T, FMT, false>(p, blocks, many, st);
 }
 
 }  // namespace
@@ -317,18 +375,21 @@ int launch_fp4_quantize(const void *x, int x_type, int64_t rows, int cols, int64
                         uint8_t *codes, uint8_t *scales, cudaStream_t st) {
   QuantizeParams p = {};
   p.x = x; p.codes = codes; p.scales = scales;
-  p.rows = rows; p.cols = cols; p.ld = ld;
+  p.rows = (uint32_t)rows; p.cols = cols; p.ld = ld;
   p.pitch = fp4_pitch(cols);
   p.tiles = fp4_tiles(cols, format);
-  p.exponent = exponent;
+  p.tensor_scale = ldexpf(1.f, exponent);
+  p.sixth = ldexpf(1.f / 6.f, -exponent);
+  p.sixth_rest = (float)ldexp(1.0 / 6.0 - (double)(1.f / 6.f), -exponent);
   if (px) {
     p.px = *px;
     p.by_OH = fp4_div((uint32_t)px->OH); p.by_OW = fp4_div((uint32_t)px->OW);
   }
+  const bool nv = format == TETRIS_FP4_NV, strided = px != nullptr;
   switch (x_type) {
-    case TETRIS_FP32: return quantize<float>(p, format, px != nullptr, st);
-    case TETRIS_BF16: return quantize<__nv_bfloat16>(p, format, px != nullptr, st);
-    default: return quantize<__half>(p, format, px != nullptr, st);
+    case TETRIS_FP32: return nv ? quantize<float, TETRIS_FP4_NV>(p, strided, st) : quantize<float, TETRIS_FP4_MX>(p, strided, st);
+    case TETRIS_BF16: return nv ? quantize<__nv_bfloat16, TETRIS_FP4_NV>(p, strided, st) : quantize<__nv_bfloat16, TETRIS_FP4_MX>(p, strided, st);
+    default: return nv ? quantize<__half, TETRIS_FP4_NV>(p, strided, st) : quantize<__half, TETRIS_FP4_MX>(p, strided, st);
   }
 }
 
@@ -336,14 +397,15 @@ int launch_fp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t r
                           int64_t ld, cudaStream_t st) {
   DequantizeParams p = {};
   p.codes = codes; p.scales = scales; p.y = y;
-  p.rows = rows; p.cols = cols; p.ld = ld;
+  p.rows = (uint32_t)rows; p.cols = cols; p.ld = ld;
   p.pitch = fp4_pitch(cols);
   p.tiles = fp4_tiles(cols, format);
-  p.exponent = exponent;
+  p.tensor_scale = ldexpf(1.f, exponent);
+  const bool nv = format == TETRIS_FP4_NV;
   switch (y_type) {
-    case TETRIS_FP32: return dequantize<float>(p, format, st);
-    case TETRIS_BF16: return dequantize<__nv_bfloat16>(p, format, st);
-    default: return dequantize<__half>(p, format, st);
+    case TETRIS_FP32: return nv ? dequantize<float, TETRIS_FP4_NV>(p, st) : dequantize<float, TETRIS_FP4_MX>(p, st);
+    case TETRIS_BF16: return nv ? dequantize<__nv_bfloat16, TETRIS_FP4_NV>(p, st) : dequantize<__nv_bfloat16, TETRIS_FP4_MX>(p, st);
+    default: return nv ? dequantize<__half, TETRIS_FP4_NV>(p, st) : dequantize<__half, TETRIS_FP4_MX>(p, st);
   }
 }
 
