@@ -3,19 +3,23 @@
 // tcgen05.mma with block scales: kind::mxf4 (32 values a scale, E8M0) and kind::mxf4nvf4 (16 a scale,
 // E4M3), both 64 values of K per instruction, FP32 accumulators in tensor memory.
 //
-// D[oc][row]: the M side is 128 output channels (the filter), the N side 16 to 256 rows.  A lane of
-// tensor memory then is a channel, so 32 lanes store 32 neighbouring values of an output row: whole lines
-// without staging, for any row distance and alignment, and few rows cost a narrow N, not an empty M.
-//   * warp 0 (one thread): per K step of 256 TMA loads of 128 filter rows and of the tile's rows (128
-//     bytes each, 128-byte swizzle, zeros past both ends) and bulk copies of the scales, into one ring;
+// Which operand is on the M side (128 lanes of tensor memory) depends on the number of rows.
+//   Few rows: the filter, D[oc][row].  16 to 64 rows cost a narrow N instead of an empty M; a lane is a channel,
+//   and 32 lanes store 32 neighbouring values of an output row.
+//   Many rows: the rows, D[row][oc].  A lane then holds neighbouring values of its row and stores 32 bytes at a
+//   time.
+// Roles:
+//   * warp 0 (one thread): per K step of 256 TMA loads of the tile's codes (128 bytes a row, 128-byte swizzle,
+//     zeros past both ends) and bulk copies of the scales, into one ring;
 //   * warp 1 (one elected lane): scales from shared into tensor memory (tcgen05.cp), then 4 MMAs;
 //   * eight storing warps: accumulator -> scale, bias, ReLU -> output, beside the next tile's MMAs.
-// Tensor memory: two accumulators.  With 256 rows two of them and the scales exceed 512 columns, so the
+// Tensor memory: two accumulators.  With N = 256 two of them and the scales exceed 512 columns, so the
 // second one lies over the end of the first; the storing warps empty the shared columns first and the next
 // tile starts once those are free.
 // Scales lie in slots of tensor memory that are written again only when the MMAs that read them are done.
-// Few tiles: the K range is cut over a cluster of up to 8 CTAs, whose sums are pushed into the shared
-// memory of the CTA that owns a row and added in slice order (bit-reproducible, no workspace).
+// Few tiles: the K range is cut over a cluster of up to 8 CTAs, whose sums are pushed into the shared memory
+// of the CTA that owns a column (asynchronous stores that count on its barrier) and added in slice order:
+// bit-reproducible, no workspace.
 // Every barrier wait is bounded; on a timeout an error flag is raised, all roles drain, tensor memory is
 // freed and the kernel returns; tetris_fp4_filter_check reports it.
 #include <cuda_bf16.h>
@@ -28,34 +32,37 @@
 namespace tetris {
 namespace {
 
-constexpr int kChannels = 128;           // channels of a tile
+constexpr int kM = 128;                  // lanes of a tile
 constexpr int kStep = 256;               // K values of a step: 128 bytes of codes
 constexpr int kStoreWarps = 8, kFirstStore = 2, kThreads = 32 * (kFirstStore + kStoreWarps);
 constexpr int kStagesMax = 8, kSlotsMax = 8;
 constexpr int kBars = 2 * kStagesMax + 8;
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kTmemCols = 512;
+constexpr int kSumPitch = kM + 1;        // floats between the columns of a cluster's sums (odd: read along either side)
+constexpr int kBiasBytes = kStoreWarps * 32 * 4;
 // Scale tiles (512 bytes, 128 rows x 4 blocks) of a K step
 __host__ __device__ constexpr int step_tiles(int format) { return format == TETRIS_FP4_NV ? 4 : 2; }
 
 struct ProductParams {
-  const uint8_t *scales_a, *scales_w;
+  const uint8_t *scales_m, *scales_n;
   const float *bias;
   void *y;
   int64_t ld;
-  int rows, N;
+  int m_extent, n_extent;  // rows and channels, or channels and rows
+  int m_blocks, n_blocks;  // 128-row blocks of either side's scales
   int steps, last_mmas;    // K steps; MMAs of the last one
-  int tiles_k;             // scale tiles of 128 rows
-  int nt;                  // rows of a tile = N of the MMAs
-  int row_tiles_128;       // 128-row blocks of the activations' scales
-  int oc_tiles, row_tiles, group;  // tiles; channel tiles that are walked side by side
+  int tiles_k;             // scale tiles of a 128-row block
+  int nt;                  // N of the MMAs
+  int m_tiles, n_tiles, group;  // tiles; M tiles that are walked side by side
   int total_tiles;
-  int d;                   // CTAs of a cluster = slices of a tile's K range
+  int d, per_log;          // CTAs of a cluster = slices of a tile's K range; log2 of the columns a CTA owns
   int stages, slots;
-  int stage_bytes, a_at, sw_at, sa_at;  // a stage: filter codes, activation codes, filter scales, activation scales
+  int stage_bytes, n_at, sm_at, sn_at;  // a stage: codes of M and N, scales of M and N
   int acc1, sf, slot_cols; // columns of the second accumulator, the scales, of a slot of them
-  float scale0, scale1;    // 2^(sum of the exponents) as two factors
+  float scale, scale1;     // 2^(sum of the exponents), as two factors where one would leave FP32
   int relu;
+  int vec;                 // bytes of an aligned store: 32, 16, or 0
   int *error_flag;
   unsigned spin_limit;
   int withhold_first_load; // failure-detection test only
@@ -147,40 +154,81 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
                : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {  // `addr` of this CTA in CTA `rank` of the cluster
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// a store into another CTA's shared memory that counts its 4 bytes on a barrier there
+__device__ __forceinline__ void st_async(uint32_t addr, uint32_t v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
 }
 template <typename T> __device__ __forceinline__ T to_type(float v);
 template <> __device__ __forceinline__ float to_type(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 to_type(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half to_type(float v) { return __float2half_rn(v); }
 
-// Tile t: channel tiles in groups of `group`, within a group all row tiles, within a row tile the group's
-// channels: CTAs that run side by side share rows and the group's part of the filter.
-__device__ __forceinline__ void decode(const ProductParams &p, int t, int &oc0, int &row0) {
-  const int per = p.group * p.row_tiles, g = t / per, r = t - g * per;
-  const int width = min(p.group, p.oc_tiles - g * p.group);
-  row0 = r / width;
-  oc0 = (g * p.group + r - row0 * width) * kChannels;
-  row0 *= p.nt;
+// Tile t: M tiles in groups of `group`, within a group all N tiles, within an N tile the group's M tiles: CTAs
+// that run side by side share both operands.
+__device__ __forceinline__ void decode(const ProductParams &p, int t, int &m0, int &n0) {
+  if (p.n_tiles == 1) {
+    m0 = t * kM; n0 = 0;
+    return;
+  }
+  const int per = p.group * p.n_tiles, g = t / per, r = t - g * per;
+  const int width = min(p.group, p.m_tiles - g * p.group);
+  n0 = r / width;
+  m0 = (g * p.group + r - n0 * width) * kM;
+  n0 *= p.nt;
 }
 
-template <int FMT, typename T>
+__device__ __forceinline__ float finish(uint32_t v, float scale, float bias, int relu) {
+  float u = fmaf(__uint_as_float(v), scale, bias);  // (the product by a power of two is exact)
+  if (relu) asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(u));
+  return u;
+}
+
+// D[row][oc]: 32 neighbouring values of a row.
+template <typename T> __device__ __forceinline__ void store_row(T *y, const float (&u)[32], int left, int vec) {
+  if (left >= 32 && vec) {
+    constexpr int kWords = 8 * sizeof(T);  // 32 values as 32-bit words
+    alignas(16) T out[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) out[j] = to_type<T>(u[j]);
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(out);
+    uint32_t *q = reinterpret_cast<uint32_t *>(y);
+    if (vec == 32) {
+#pragma unroll
+      for (int j = 0; j < kWords; j += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(q + j), "r"(w[j]), "r"(w[j + 1]), "r"(w[j + 2]), "r"(w[j + 3]),
+                     "r"(w[j + 4]), "r"(w[j + 5]), "r"(w[j + 6]), "r"(w[j + 7]) : "memory");
+    } else {
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4) *reinterpret_cast<uint4 *>(q + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) y[j] = to_type<T>(u[j]);
+  }
+}
+
+template <int FMT, typename T, bool ROWS_M>
 __global__ void __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const ProductParams p) {
+product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const ProductParams p) {
   constexpr int kTiles = step_tiles(FMT);
   extern __shared__ unsigned char smem_raw[];
   unsigned char *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  unsigned char *tail = ring + (size_t)p.stages * p.stage_bytes;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(tail);
+  float *sums = reinterpret_cast<float *>(ring + (size_t)p.stages * p.stage_bytes);   // d > 1: [slice][column][kSumPitch]
+  float *bias_rows = sums + (p.d > 1 ? p.nt * kSumPitch : 0);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(bias_rows) + kBiasBytes);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -190,16 +238,57 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   auto bar_pempty = [&](int b) { return smem_u32(&bars[2 * kStagesMax + 2 + b]); };
   auto bar_shared = [&](int b) { return smem_u32(&bars[2 * kStagesMax + 4 + b]); };
   auto bar_drain = [&]() { return smem_u32(&bars[2 * kStagesMax + 6]); };
+  auto bar_sums = [&]() { return smem_u32(&bars[2 * kStagesMax + 7]); };
+
+  const int rank = p.d > 1 ? (int)(blockIdx.x & (p.d - 1)) : 0;
+  const int tile0 = p.d > 1 ? blockIdx.x / p.d : blockIdx.x, tile_step = p.d > 1 ? gridDim.x / p.d : gridDim.x;
+  const int step0 = p.d > 1 ? (int)((int64_t)p.steps * rank / p.d) : 0, step1 = p.d > 1 ? (int)((int64_t)p.steps * (rank + 1) / p.d) : p.steps;
+  const int rt = p.nt > 128 ? 2 : 1;       // 128-row blocks of a tile's N scales
+  const bool over = p.acc1 < p.nt;         // the accumulators share columns
+  const int ahead = min(step1 - step0, p.stages);
+  int loads = 0;
+  int m0, n0;
+
+  // Bytes of a step: both code boxes whole (zeros past the ends count), the scale tiles that exist.  The filter
+  // does not change while kernels run, the activations may until grid_wait.
+  auto scale_tiles = [&](int step) { return min(kTiles, p.tiles_k - step * kTiles); };
+  auto load_m = [&](uint32_t at, uint32_t bar, int step) {
+    tma_load_2d(at, &map_m, bar, step * 128, m0);
+    bulk_load(at + p.sm_at, p.scales_m + ((size_t)(m0 / 128) * p.tiles_k + (size_t)step * kTiles) * 512, scale_tiles(step) * 512, bar);
+  };
+  auto load_n = [&](uint32_t at, uint32_t bar, int step) {
+    const int b0 = n0 / 128, blocks = min(rt, p.n_blocks - b0);
+    tma_load_2d(at + p.n_at, &map_n, bar, step * 128, n0);
+    for (int b = 0; b < blocks; ++b)
+      bulk_load(at + p.sn_at + b * (kTiles * 512), p.scales_n + ((size_t)(b0 + b) * p.tiles_k + (size_t)step * kTiles) * 512, scale_tiles(step) * 512, bar);
+  };
+  auto load_filter = [&](int s, int step) {
+    const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
+    mbar_expect_tx(bar, (uint32_t)((kM + p.nt) * 128 + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
+    if (ROWS_M) load_n(at, bar, step); else load_m(at, bar, step);
+  };
+  auto load_rows = [&](int s, int step) {
+    const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
+    if (loads++ == 0 && p.withhold_first_load) return;  // (test: that step never arrives, its reader gives up)
+    if (ROWS_M) load_m(at, bar, step); else load_n(at, bar, step);
+  };
 
   if (tid == 0) {
     for (int s = 0; s < kStagesMax; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(bar_pfull(b), 1); mbar_init(bar_pempty(b), kStoreWarps); mbar_init(bar_shared(b), kStoreWarps); }
     mbar_init(bar_drain(), 1);
+    mbar_init(bar_sums(), 1);
     abort_flag[0] = 0;
     abort_flag[1] = (int)(p.spin_limit ? p.spin_limit : kSpinLimit);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // the filter's part of the empty ring is sent for while the launch before this one drains
+    decode(p, tile0, m0, n0);
+    for (int i = 0; i < ahead; ++i) load_filter(i, step0 + i);
+    if (p.d > 1) {
+      const int live = min(p.nt, p.n_extent - n0) - (rank << p.per_log);  // columns that this CTA adds up
+      mbar_expect_tx(bar_sums(), (uint32_t)(max(0, min(1 << p.per_log, live)) * p.d * kM * 4));
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
@@ -208,63 +297,30 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (p.d > 1) cluster_arrive();  // (waited for before anything reaches into another CTA)
   const uint32_t tmem = *tmem_slot;
   if (tid == 0) grid_release();  // (this CTA has its tensor memory: nothing it waits for can be held by the next launch)
-  if (warp != 0) grid_wait();    // (warp 0 sends for the filter first)
-
-  const int rank = p.d > 1 ? (int)(blockIdx.x % p.d) : 0;
-  const int tile0 = blockIdx.x / p.d, tile_step = gridDim.x / p.d;
-  const int step0 = (int)((int64_t)p.steps * rank / p.d), step1 = (int)((int64_t)p.steps * (rank + 1) / p.d);
-  const int rt = p.nt > 128 ? 2 : 1;       // 128-row blocks of a tile's scales
-  const bool over = p.acc1 < p.nt;         // the accumulators share columns
-  int loads = 0;
+  grid_wait();
 
   if (warp == 0) {
     if (lane == 0) {
-      int oc0, row0;
-      // Bytes of a step: both code boxes whole (zeros past the ends count), the scale tiles that exist.
-      auto scale_tiles = [&](int step) { return min(kTiles, p.tiles_k - step * kTiles); };
-      auto load_w = [&](int s, int step) {
-        const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-        const int n = scale_tiles(step), blocks = min(rt, p.row_tiles_128 - row0 / 128);
-        mbar_expect_tx(bar, (uint32_t)((kChannels + p.nt) * 128 + n * 512 * (1 + blocks)));
-        tma_load_2d(at, &map_w, bar, step * 128, oc0);
-        bulk_load(at + p.sw_at, p.scales_w + ((size_t)(oc0 / 128) * p.tiles_k + (size_t)step * kTiles) * 512, n * 512, bar);
-      };
-      auto load_a = [&](int s, int step) {
-        const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-        const int n = scale_tiles(step), b0 = row0 / 128, blocks = min(rt, p.row_tiles_128 - b0);
-        if (loads++ == 0 && p.withhold_first_load) return;  // (test: that step never arrives, its reader gives up)
-        tma_load_2d(at + p.a_at, &map_a, bar, step * 128, row0);
-        for (int b = 0; b < blocks; ++b)
-          bulk_load(at + p.sa_at + b * (kTiles * 512), p.scales_a + ((size_t)(b0 + b) * p.tiles_k + (size_t)step * kTiles) * 512, n * 512, bar);
-      };
-      int s = 0;
-      uint32_t parity = 1;  // of the empty barriers
+      for (int i = 0; i < ahead; ++i) load_rows(i, step0 + i);
+      int s = ahead == p.stages ? 0 : ahead;
+      uint32_t parity = ahead == p.stages ? 0 : 1;  // of the empty barriers
       bool ok = true;
       for (int t = tile0; t < p.total_tiles && ok; t += tile_step) {
-        decode(p, t, oc0, row0);
-        int step = step0;
-        if (t == tile0) {  // the ring is empty: the filter's part is sent for while the launch before this one drains
-          const int ahead = min(step1 - step0, p.stages);
-          for (int i = 0; i < ahead; ++i) load_w(i, step0 + i);
-          grid_wait();
-          for (int i = 0; i < ahead; ++i) load_a(i, step0 + i);
-          step += ahead;
-          s = ahead;
-          if (s == p.stages) { s = 0; parity ^= 1; }
-        }
-        for (; step < step1; ++step) {
+        if (t != tile0) decode(p, t, m0, n0);
+        for (int step = t == tile0 ? step0 + ahead : step0; step < step1; ++step) {
           if (!(ok = mbar_wait(bar_empty(s), parity, abort_flag))) break;
-          load_w(s, step);
-          load_a(s, step);
+          load_filter(s, step);
+          load_rows(s, step);
           if (++s == p.stages) { s = 0; parity ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
     // The loop has no early exits: a wait that gave up raises the abort flag, later waits then return at once.
-    constexpr uint32_t kFormats = (1u << 7) | (1u << 10) | (FMT == TETRIS_FP4_NV ? 0u : 1u << 23) | ((uint32_t)(kChannels >> 4) << 24);
+    constexpr uint32_t kFormats = (1u << 7) | (1u << 10) | (FMT == TETRIS_FP4_NV ? 0u : 1u << 23) | ((uint32_t)(kM >> 4) << 24);
     const uint32_t idesc = kFormats | ((uint32_t)(p.nt >> 3) << 17);
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
@@ -274,11 +330,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     uint32_t parity = 0, free_parity = 0;
     int i = 0;
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
-      int oc0, row0;
-      decode(p, t, oc0, row0);
+      decode(p, t, m0, n0);
       const int b = i & 1;
       const uint32_t acc = tmem + (b ? p.acc1 : 0);
-      const uint32_t sf_row = (uint32_t)(row0 & 127) >> 5;   // the tile's first 32-row group within its scale tile: 0 or 2
+      const uint32_t sf_row = (uint32_t)(n0 & 127) >> 5;   // the tile's first 32-row group within its scale tile: 0 or 2
       if (i >= 2) wait(bar_pempty(b), ((i >> 1) & 1) ^ 1);
       if (over && i >= 1) wait(bar_shared(b ^ 1), ((i - 1) >> 1) & 1);
       for (int step = step0; step < step1; ++step) {
@@ -290,25 +345,25 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         wait(bar_full(s), parity);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes);
-        const uint32_t sfw = tmem + p.sf + slot * p.slot_cols, sfa = sfw + 4 * kTiles;
+        const uint32_t sfm = tmem + p.sf + slot * p.slot_cols, sfn = sfm + 4 * kTiles;
         const int n = min(kTiles, p.tiles_k - step * kTiles), mmas = step == p.steps - 1 ? p.last_mmas : 4;
         if (elect_one()) {
-          const uint64_t dsw = scales_desc(at + p.sw_at), dsa = scales_desc(at + p.sa_at);
+          const uint64_t dsm = scales_desc(at + p.sm_at), dsn = scales_desc(at + p.sn_at);
 #pragma unroll
           for (int k = 0; k < kTiles; ++k) {
             if (k < n) {
-              copy_scales(sfw + 4 * k, dsw + 32 * k);
-              copy_scales(sfa + 4 * rt * k, dsa + 32 * k);
-              if (rt == 2) copy_scales(sfa + 8 * k + 4, dsa + 32 * (kTiles + k));
+              copy_scales(sfm + 4 * k, dsm + 32 * k);
+              copy_scales(sfn + 4 * rt * k, dsn + 32 * k);
+              if (rt == 2) copy_scales(sfn + 8 * k + 4, dsn + 32 * (kTiles + k));
             }
           }
-          const uint64_t dw = codes_desc(at), da = codes_desc(at + p.a_at);
+          const uint64_t dm = codes_desc(at), dn = codes_desc(at + p.n_at);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j < mmas) {
               const int k = FMT == TETRIS_FP4_NV ? j : j >> 1;
               const uint32_t id = FMT == TETRIS_FP4_NV || !(j & 1) ? idesc : idesc | (2u << 4) | (2u << 29);  // (second half of the scale words)
-              umma_fp4<FMT>(acc, dw + 2 * j, da + 2 * j, id, sfw + 4 * k, sfa + 4 * rt * k + sf_row, step > step0 || j > 0);
+              umma_fp4<FMT>(acc, dm + 2 * j, dn + 2 * j, id, sfm + 4 * k, sfn + 4 * rt * k + sf_row, step > step0 || j > 0);
             }
           }
           umma_commit(bar_empty(s));
@@ -320,22 +375,21 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         if (++slot == p.slots) slot = 0;
       }
     }
-  } else {
+  } else if (p.d == 1) {
     const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;
     const int chunks = (p.nt + 31) / 32, shared = over ? (p.nt - p.acc1) / 32 : 0;
+    float *bias_row = bias_rows + (warp - kFirstStore) * 32;
     int i = 0;
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
-      int oc0, row0;
-      decode(p, t, oc0, row0);
-      const int b = i & 1;
+      decode(p, t, m0, n0);
+      const int b = i & 1, m = m0 + quarter * 32 + lane;
       if (!mbar_try_wait(bar_pfull(b), (i >> 1) & 1)) mbar_wait(bar_pfull(b), (i >> 1) & 1, abort_flag);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (p.d > 1) break;  // a slice of a tile: its sums stay in tensor memory until the cluster meets
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (b ? p.acc1 : 0);
-      const int oc = oc0 + quarter * 32 + lane;
-      const float bias = p.bias && oc < p.N ? p.bias[oc] : 0.f;
+      const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
       bool told = !over;
+#pragma unroll 1
       for (int c = half; c < chunks; c += 2) {
         const int chunk = b ? c : chunks - 1 - c;  // the shared columns: the first accumulator's last, the second one's first
         if (!told && c >= shared) {
@@ -345,14 +399,37 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           told = true;
         }
         uint32_t v[32];
+        const int n = n0 + chunk * 32;
+        if (ROWS_M && p.bias) {
+          __syncwarp();
+          bias_row[lane] = n + lane < p.n_extent ? p.bias[n + lane] : 0.f;
+          __syncwarp();
+        }
         tmem_ld32(acc + chunk * 32, v);
-        const int row = row0 + chunk * 32, n = oc < p.N ? p.rows - row : 0;
-        T *y = static_cast<T *>(p.y) + (int64_t)row * p.ld + oc;
+        if (p.scale1 != 1.f) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float u = __uint_as_float(v[j]) * p.scale0 * p.scale1 + bias;
-          if (p.relu && u < 0.f) u = 0.f;  // (a NaN stays)
-          if (j < n) y[j * p.ld] = to_type<T>(u);
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * p.scale1);
+        }
+        if (ROWS_M) {
+          float u[32];
+          if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 bb = *reinterpret_cast<const float4 *>(bias_row + j);
+              u[j] = finish(v[j], p.scale, bb.x, p.relu); u[j + 1] = finish(v[j + 1], p.scale, bb.y, p.relu);
+              u[j + 2] = finish(v[j + 2], p.scale, bb.z, p.relu); u[j + 3] = finish(v[j + 3], p.scale, bb.w, p.relu);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = finish(v[j], p.scale, 0.f, p.relu);
+          }
+          if (m < p.m_extent) store_row<T>(static_cast<T *>(p.y) + (int64_t)m * p.ld + n, u, p.n_extent - n, p.vec);
+        } else {
+          const int left = m < p.m_extent ? p.n_extent - n : 0;
+          T *y = static_cast<T *>(p.y) + (int64_t)n * p.ld + m;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < left) y[j * p.ld] = to_type<T>(finish(v[j], p.scale, lane_bias, p.relu));
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -362,8 +439,49 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         mbar_arrive(bar_pempty(b));
       }
     }
+  } else {
+    // The slices of a tile meet: a CTA owns 2^per_log columns; each pushes its sums of a column (128 lanes) to
+    // the owner, who adds them up in slice order.
+    const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;
+    decode(p, tile0, m0, n0);
+    const int live = min(p.nt, p.n_extent - n0);
+    bool ok = mbar_wait(bar_pfull(0), 0, abort_flag);
+    cluster_wait();  // (every CTA of the cluster runs)
+    ok = __all_sync(0xffffffffu, ok);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (ok) {
+      const uint32_t mine = smem_u32(sums) + (uint32_t)(quarter * 32 + lane) * 4u, bar = bar_sums();
+#pragma unroll 1
+      for (int c = half * 8; c < live; c += 16) {
+        uint32_t v[8];
+        tmem_ld8(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int owner = (c + j) >> p.per_log, at = (rank << p.per_log) + (c + j - (owner << p.per_log));
+          if (c + j < live) st_async(cluster_addr(mine + (uint32_t)(at * kSumPitch) * 4u, owner), v[j], cluster_addr(bar, owner));
+        }
+      }
+    }
+    ok = __all_sync(0xffffffffu, mbar_wait(bar_sums(), 0, abort_flag)) && ok;
+    cluster_arrive();  // (what this CTA is owed has come, or it has given up; all of its own pushes are on their way)
+    const int own = ok ? min(1 << p.per_log, live - (rank << p.per_log)) : 0, own0 = n0 + (rank << p.per_log);
+    const int e0 = tid - 32 * kFirstStore;
+    // D[oc][row]: neighbouring threads take neighbouring lanes; D[row][oc]: neighbouring columns
+    for (int e = e0; e < own * kM; e += 32 * kStoreWarps) {
+      const int j = ROWS_M ? e % own : e / kM, l = ROWS_M ? e / own : e % kM;
+      if (m0 + l >= p.m_extent) continue;
+      float u = 0.f;
+      for (int s = 0; s < p.d; ++s) u += sums[((s << p.per_log) + j) * kSumPitch + l];
+      const int row = ROWS_M ? m0 + l : own0 + j, oc = ROWS_M ? own0 + j : m0 + l;
+      u = finish(__float_as_uint(u * p.scale1), p.scale, p.bias ? p.bias[oc] : 0.f, p.relu);
+      static_cast<T *>(p.y)[(int64_t)row * p.ld + oc] = to_type<T>(u);
+    }
   }
   __syncwarp();
+  if (p.d > 1 && warp < kFirstStore) {
+    cluster_wait();
+    cluster_arrive();
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -376,45 +494,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       mbar_drain(bar_drain(), 0);
     }
     if (tid == 0) atomicExch(p.error_flag, 1);
-  }
-  if (p.d > 1) {
-    // The slices of a tile meet: a CTA owns `per` rows; each pushes its sums of a row (128 channels) to the
-    // owner, once every ring of the cluster is idle, and the owner adds them up in slice order.
-    const int per = (p.nt + p.d - 1) / p.d;
-    int oc0, row0;
-    decode(p, tile0, oc0, row0);
-    const int live = min(p.nt, p.rows - row0);
-    cluster_sync_all();
-    if (warp >= kFirstStore && !*abort_flag) {
-      const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;
-      const uint32_t mine = smem_u32(ring) + (uint32_t)(quarter * 32 + lane) * 4u;
-      for (int c = half * 32; c < live; c += 64) {
-        uint32_t v[32];
-        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (c + j < live) {
-            const int owner = (c + j) / per;
-            st_cluster(cluster_addr(mine + (uint32_t)((rank * per + c + j - owner * per) * kChannels) * 4u, (uint32_t)owner), __uint_as_float(v[j]));
-          }
-        }
-      }
-    }
     __syncwarp();
-    cluster_sync_all();  // (all sums have arrived; nothing reaches into another CTA after this)
-    const float *sums = reinterpret_cast<const float *>(ring);
-    const int mine = *abort_flag ? 0 : min(per, live - rank * per);
-    for (int e = tid; e < mine * kChannels; e += kThreads) {
-      const int j = e / kChannels, c = e % kChannels, oc = oc0 + c;
-      if (oc >= p.N) continue;
-      float u = 0.f;
-      for (int s = 0; s < p.d; ++s) u += sums[(s * per + j) * kChannels + c];
-      u = u * p.scale0 * p.scale1 + (p.bias ? p.bias[oc] : 0.f);
-      if (p.relu && u < 0.f) u = 0.f;
-      static_cast<T *>(p.y)[(int64_t)(row0 + rank * per + j) * p.ld + oc] = to_type<T>(u);
-    }
   }
-  __syncthreads();
+  if (p.d > 1) cluster_wait();  // (no CTA leaves while another one may still push into it)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
@@ -433,41 +515,51 @@ constexpr size_t kSmemMost = 227 * 1024 - 1024;   // (the ring is aligned to 102
 constexpr size_t kSmemLeast = 117 * 1024;         // one CTA per SM, also beside the other kernels that take all of an SM's tensor memory
 
 struct Geometry {
+  bool rows_m;
   int nt, d;
 };
 
+// The least of an estimate in clocks: waves of tiles, each K step at the longer of its MMAs and its loads
+// (about 44 bytes a clock and SM from L2), the store of the last tile, the meeting of a cluster.
 Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
-  const int steps = (f->in_channel + kStep - 1) / kStep, oc_tiles = (f->out_channel + kChannels - 1) / kChannels;
-  Geometry best = {16, 1};
+  const int steps = (f->in_channel + kStep - 1) / kStep;
+  Geometry best = {false, 16, 1};
   double least = 1e300;
-  for (int nt = 16; nt <= 256; nt *= 2) {
-    // The scales of a tile begin at its first 32-row group's column, and an MMA takes scales from even columns
-    // only (an odd one is a misaligned address): tiles below 64 rows begin at row 0.
-    if (nt < 64 && rows > nt) continue;
-    const int64_t tiles = (rows + nt - 1) / nt * oc_tiles;
-    for (int d = 1; d <= 8; d *= 2) {
-      if (d > 1 && (d > steps || nt > 64 || tiles * d > f->sm_count)) continue;
-      const double waves = (double)((tiles * d + f->sm_count - 1) / f->sm_count);
-      const double step = std::max(2.0 * nt, (kChannels * 144 + nt * 144) / 40.0), store = 300 + 6.0 * nt;
-      const double cost = waves * ((double)((steps + d - 1) / d) * step + (d > 1 ? 2000 : 0)) + (waves > 1 ? 0 : store) + 2000;
-      if (cost < least) { least = cost; best = {nt, d}; }
+  for (int rows_m = 0; rows_m < 2; ++rows_m) {
+    const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
+    for (int nt = 16; nt <= 256; nt *= 2) {
+      // The scales of a tile begin at its first 32-row group's column, and an MMA takes scales from even columns
+      // only (an odd one is a misaligned address): tiles below 64 begin at 0.
+      if (nt < 64 && n > nt) continue;
+      const int64_t tiles = (m + kM - 1) / kM * ((n + nt - 1) / nt);
+      for (int d = 1; d <= 8; d *= 2) {
+        if (d > 1 && (d > steps || nt > 128 || tiles * d > f->sm_count)) continue;
+        const double waves = (double)((tiles * d + f->sm_count - 1) / f->sm_count);
+        const double step = std::max(2.0 * nt, (kM + nt) * 144 / 44.0), store = (rows_m ? 4.0 : 8.0) * nt;
+        const double cost = waves * std::max((double)((steps + d - 1) / d) * step, store) + (d > 1 ? 1500 + 4.0 * nt : store);
+        if (cost < least) { least = cost; best = {rows_m != 0, nt, d}; }
+      }
     }
   }
   return best;
 }
 
-template <int FMT, typename T>
-int launch(const CUtensorMap &map_w, const CUtensorMap &map_a, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
+template <int FMT, typename T, bool ROWS_M>
+int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
   static bool ready[64] = {};  // per device
   int dev = 0;
   TETRIS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024)));
+    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024)));
     if (dev < 64) ready[dev] = true;
   }
-  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_w, map_a, p));
+  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, p));
   count_launch();
   return TETRIS_OK;
+}
+template <int FMT, typename T>
+int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
+  return rows_m ? launch<FMT, T, true>(map_m, map_n, p, grid, smem, st) : launch<FMT, T, false>(map_m, map_n, p, grid, smem, st);
 }
 
 int encode(CUtensorMap *map, const uint8_t *codes, int64_t pitch, int64_t rows, int box_rows) {
@@ -487,46 +579,51 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
                        void *y, int y_type, int64_t ld, int relu, cudaStream_t st) {
   const Geometry g = choose(f, rows);
   const bool nv = f->format == TETRIS_FP4_NV;
-  const int kt = step_tiles(f->format), rt = g.nt > 128 ? 2 : 1;
+  const int kt = step_tiles(f->format), rt = g.nt > 128 ? 2 : 1, bytes = y_type == TETRIS_FP32 ? 4 : 2;
   ProductParams p = {};
-  p.scales_a = scales; p.scales_w = f->d_scales; p.bias = bias;
+  p.scales_m = g.rows_m ? scales : f->d_scales; p.scales_n = g.rows_m ? f->d_scales : scales;
+  p.bias = bias;
   p.y = y; p.ld = ld;
-  p.rows = (int)rows; p.N = f->out_channel;
+  p.m_extent = (int)(g.rows_m ? rows : f->out_channel); p.n_extent = (int)(g.rows_m ? f->out_channel : rows);
+  p.m_blocks = (p.m_extent + 127) / 128; p.n_blocks = (p.n_extent + 127) / 128;
   p.steps = (f->in_channel + kStep - 1) / kStep;
   p.last_mmas = (f->in_channel - (p.steps - 1) * kStep + 63) / 64;
   p.tiles_k = fp4_tiles(f->in_channel, f->format);
   p.nt = g.nt; p.d = g.d;
-  p.row_tiles_128 = (int)((rows + 127) / 128);
-  p.oc_tiles = (f->out_channel + kChannels - 1) / kChannels;
-  p.row_tiles = (int)((rows + g.nt - 1) / g.nt);
-  p.group = std::min(p.oc_tiles, 8);
-  const int64_t total = (int64_t)p.oc_tiles * p.row_tiles;
+  for (p.per_log = 0; g.nt / g.d >> (p.per_log + 1); ++p.per_log) {}
+  p.m_tiles = p.m_blocks;
+  p.n_tiles = (p.n_extent + g.nt - 1) / g.nt;
+  p.group = std::min(p.m_tiles, 16);
+  const int64_t total = (int64_t)p.m_tiles * p.n_tiles;
   if (total > 0x3FFFFFFF) { set_error("a product of %lld tiles is outside what the kernels cover", (long long)total); return TETRIS_ERR_UNSUPPORTED; }
   p.total_tiles = (int)total;
-  p.a_at = kChannels * 128;
-  p.sw_at = p.a_at + std::max(g.nt * 128, 2048);
-  p.sa_at = p.sw_at + kt * 512;
-  p.stage_bytes = (p.sa_at + rt * kt * 512 + 1023) / 1024 * 1024;
-  const size_t tail = kBars * 8 + 16;
+  p.n_at = kM * 128;
+  p.sm_at = p.n_at + g.nt * 128;
+  p.sn_at = p.sm_at + kt * 512;
+  p.stage_bytes = (p.sn_at + rt * kt * 512 + 1023) / 1024 * 1024;
+  const size_t tail = (g.d > 1 ? (size_t)g.nt * kSumPitch * 4 : 0) + kBiasBytes + kBars * 8 + 16;
   p.stages = std::min<int>(kStagesMax, (int)((kSmemMost - tail) / p.stage_bytes));
   p.slot_cols = 4 * kt * (1 + rt);
   p.slots = rt == 2 ? 2 : std::min(kSlotsMax, p.stages);  // (at most `stages`: a step's empty barrier is waited for before the stage is used again)
   p.sf = kTmemCols - p.slots * p.slot_cols;
   p.acc1 = std::min(std::max(g.nt, 32), (p.sf - g.nt) / 32 * 32);
   const int e = exponent + f->exponent, e0 = std::max(-126, std::min(126, e));
-  p.scale0 = ldexpf(1.f, e0); p.scale1 = ldexpf(1.f, e - e0);
+  p.scale = ldexpf(1.f, e0); p.scale1 = ldexpf(1.f, e - e0);
   p.relu = relu;
+  for (p.vec = 32; p.vec >= 16 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes)) & (p.vec - 1)); p.vec /= 2) {}
+  if (p.vec < 16) p.vec = 0;
   p.error_flag = f->d_error;
   p.withhold_first_load = test_injection(&p.spin_limit);
   CUtensorMap map_w, map_a;
   int rc;
-  if ((rc = encode(&map_w, f->d_codes, f->pitch, f->out_channel, kChannels)) || (rc = encode(&map_a, codes, f->pitch, rows, g.nt))) return rc;
+  if ((rc = encode(&map_w, f->d_codes, f->pitch, f->out_channel, g.rows_m ? g.nt : kM)) || (rc = encode(&map_a, codes, f->pitch, rows, g.rows_m ? kM : g.nt))) return rc;
+  const CUtensorMap &map_m = g.rows_m ? map_a : map_w, &map_n = g.rows_m ? map_w : map_a;
   const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, f->sm_count));
   const size_t smem = std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail + 1024);
   switch (y_type) {
-    case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(map_w, map_a, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(map_w, map_a, p, grid, smem, st);
-    case TETRIS_BF16: return nv ? launch<TETRIS_FP4_NV, __nv_bfloat16>(map_w, map_a, p, grid, smem, st) : launch<TETRIS_FP4_MX, __nv_bfloat16>(map_w, map_a, p, grid, smem, st);
-    default: return nv ? launch<TETRIS_FP4_NV, __half>(map_w, map_a, p, grid, smem, st) : launch<TETRIS_FP4_MX, __half>(map_w, map_a, p, grid, smem, st);
+    case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, p, grid, smem, st);
+    case TETRIS_BF16: return nv ? launch<TETRIS_FP4_NV, __nv_bfloat16>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, __nv_bfloat16>(g.rows_m, map_m, map_n, p, grid, smem, st);
+    default: return nv ? launch<TETRIS_FP4_NV, __half>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, __half>(g.rows_m, map_m, map_n, p, grid, smem, st);
   }
 }
 
