@@ -39,8 +39,9 @@ constexpr int kStagesMax = 8, kSlotsMax = 8;
 constexpr int kBars = 2 * kStagesMax + 8;
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kTmemCols = 512;
-constexpr int kSumPitch = kM + 1;        // floats between the columns of a cluster's sums (odd: read along either side)
-constexpr int kBiasBytes = kStoreWarps * 32 * 4;
+constexpr int kSumPitch = kM + 4;        // floats between the columns of a cluster's sums (whole 16 bytes)
+constexpr int kBiasBytes = kStoreWarps * 64 * 4;
+constexpr int kStageOut = 4096;          // a staging block: 32 rows of 128 bytes on their way to the output
 // Scale tiles (512 bytes, 128 rows x 4 blocks) of a K step
 __host__ __device__ constexpr int step_tiles(int format) { return format == TETRIS_FP4_NV ? 4 : 2; }
 
@@ -55,6 +56,7 @@ struct ProductParams {
   int tiles_k;             // scale tiles of a 128-row block
   int nt;                  // N of the MMAs
   int m_tiles, n_tiles, group;  // tiles; M tiles that are walked side by side
+  Fp4Div by_per, by_group, by_last;  // tiles of a group of M tiles; its M tiles; those of the last group
   int total_tiles;
   int d, per_log;          // CTAs of a cluster = slices of a tile's K range; log2 of the columns a CTA owns
   int stages, slots;
@@ -62,7 +64,8 @@ struct ProductParams {
   int acc1, sf, slot_cols; // columns of the second accumulator, the scales, of a slot of them
   float scale, scale1;     // 2^(sum of the exponents), as two factors where one would leave FP32
   int relu;
-  int vec;                 // bytes of an aligned store: 32, 16, or 0
+  int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows)
+  int staging;             // ... staging blocks of a storing warp: 1 or 2
   int *error_flag;
   unsigned spin_limit;
   int withhold_first_load; // failure-detection test only
@@ -154,11 +157,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
                : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {  // `addr` of this CTA in CTA `rank` of the cluster
@@ -166,9 +164,12 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-// a store into another CTA's shared memory that counts its 4 bytes on a barrier there
-__device__ __forceinline__ void st_async(uint32_t addr, uint32_t v, uint32_t bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
+// shared memory of this CTA into another one's, counted on a barrier there
+__device__ __forceinline__ void push(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
 template <typename T> __device__ __forceinline__ T to_type(float v);
 template <> __device__ __forceinline__ float to_type(float v) { return v; }
@@ -178,15 +179,11 @@ template <> __device__ __forceinline__ __half to_type(float v) { return __float2
 // Tile t: M tiles in groups of `group`, within a group all N tiles, within an N tile the group's M tiles: CTAs
 // that run side by side share both operands.
 __device__ __forceinline__ void decode(const ProductParams &p, int t, int &m0, int &n0) {
-  if (p.n_tiles == 1) {
-    m0 = t * kM; n0 = 0;
-    return;
-  }
-  const int per = p.group * p.n_tiles, g = t / per, r = t - g * per;
-  const int width = min(p.group, p.m_tiles - g * p.group);
-  n0 = r / width;
-  m0 = (g * p.group + r - n0 * width) * kM;
-  n0 *= p.nt;
+  const int g = (int)fp4_quot((uint32_t)t, p.by_per), r = t - g * (int)p.by_per.d;
+  const Fp4Div &w = (g + 1) * p.group <= p.m_tiles ? p.by_group : p.by_last;
+  const int n = (int)fp4_quot((uint32_t)r, w);
+  m0 = (g * p.group + r - n * (int)w.d) * kM;
+  n0 = n * p.nt;
 }
 
 __device__ __forceinline__ float finish(uint32_t v, float scale, float bias, int relu) {
@@ -195,39 +192,17 @@ __device__ __forceinline__ float finish(uint32_t v, float scale, float bias, int
   return u;
 }
 
-// D[row][oc]: 32 neighbouring values of a row.
-template <typename T> __device__ __forceinline__ void store_row(T *y, const float (&u)[32], int left, int vec) {
-  if (left >= 32 && vec) {
-    constexpr int kWords = 8 * sizeof(T);  // 32 values as 32-bit words
-    alignas(16) T out[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) out[j] = to_type<T>(u[j]);
-    const uint32_t *w = reinterpret_cast<const uint32_t *>(out);
-    uint32_t *q = reinterpret_cast<uint32_t *>(y);
-    if (vec == 32) {
-#pragma unroll
-      for (int j = 0; j < kWords; j += 8)
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(q + j), "r"(w[j]), "r"(w[j + 1]), "r"(w[j + 2]), "r"(w[j + 3]),
-                     "r"(w[j + 4]), "r"(w[j + 5]), "r"(w[j + 6]), "r"(w[j + 7]) : "memory");
-    } else {
-#pragma unroll
-      for (int j = 0; j < kWords; j += 4) *reinterpret_cast<uint4 *>(q + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < left) y[j] = to_type<T>(u[j]);
-  }
-}
-
 template <int FMT, typename T, bool ROWS_M>
 __global__ void __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const ProductParams p) {
+product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const __grid_constant__ CUtensorMap map_y,
+               const ProductParams p) {
   constexpr int kTiles = step_tiles(FMT);
   extern __shared__ unsigned char smem_raw[];
   unsigned char *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float *sums = reinterpret_cast<float *>(ring + (size_t)p.stages * p.stage_bytes);   // d > 1: [slice][column][kSumPitch]
-  float *bias_rows = sums + (p.d > 1 ? p.nt * kSumPitch : 0);
+  // behind the ring: staging blocks (D[row][oc]), or, for d > 1, the sums of this CTA's columns [slice][column][kSumPitch]
+  unsigned char *staging = ring + (size_t)p.stages * p.stage_bytes;
+  float *sums = reinterpret_cast<float *>(staging);
+  float *bias_rows = reinterpret_cast<float *>(staging + (p.d > 1 ? p.nt * kSumPitch * 4 : kStoreWarps * kStageOut * p.staging));
   uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(bias_rows) + kBiasBytes);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -287,7 +262,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     for (int i = 0; i < ahead; ++i) load_filter(i, step0 + i);
     if (p.d > 1) {
       const int live = min(p.nt, p.n_extent - n0) - (rank << p.per_log);  // columns that this CTA adds up
-      mbar_expect_tx(bar_sums(), (uint32_t)(max(0, min(1 << p.per_log, live)) * p.d * kM * 4));
+      mbar_expect_tx(bar_sums(), (uint32_t)(max(0, min(1 << p.per_log, live)) * p.d * kSumPitch * 4));
     }
   }
   if (warp == 1) {
@@ -376,62 +351,108 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       }
     }
   } else if (p.d == 1) {
-    const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;
-    const int chunks = (p.nt + 31) / 32, shared = over ? (p.nt - p.acc1) / 32 : 0;
-    float *bias_row = bias_rows + (warp - kFirstStore) * 32;
+    constexpr int kUnit = ROWS_M ? 128 / (int)sizeof(T) : 32;   // columns that a warp takes at a time (D[row][oc]: 128 bytes of a row)
+    const int me = warp - kFirstStore, quarter = warp & 3, half = me >> 2;
+    const int units = max(1, p.nt / kUnit), shared = over ? (p.nt - p.acc1 + kUnit - 1) / kUnit : 0;
+    float *bias_row = bias_rows + me * 64;
+    unsigned char *blocks = staging + me * kStageOut * p.staging;
+    int nblk = 0;
     int i = 0;
+    decode(p, tile0, m0, n0);
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
-      decode(p, t, m0, n0);
-      const int b = i & 1, m = m0 + quarter * 32 + lane;
+      const int b = i & 1, mq = m0 + quarter * 32, m = mq + lane, n_first = n0;
+      const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
       if (!mbar_try_wait(bar_pfull(b), (i >> 1) & 1)) mbar_wait(bar_pfull(b), (i >> 1) & 1, abort_flag);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (b ? p.acc1 : 0);
-      const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
       bool told = !over;
 #pragma unroll 1
-      for (int c = half; c < chunks; c += 2) {
-        const int chunk = b ? c : chunks - 1 - c;  // the shared columns: the first accumulator's last, the second one's first
+      for (int c = half; c < units; c += 2) {
+        const int unit = b ? c : units - 1 - c;  // the shared columns: the first accumulator's last, the second one's first
         if (!told && c >= shared) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_shared(b));
           told = true;
         }
+        const int n = n_first + unit * kUnit;
         uint32_t v[32];
-        const int n = n0 + chunk * 32;
-        if (ROWS_M && p.bias) {
-          __syncwarp();
-          bias_row[lane] = n + lane < p.n_extent ? p.bias[n + lane] : 0.f;
-          __syncwarp();
-        }
-        tmem_ld32(acc + chunk * 32, v);
-        if (p.scale1 != 1.f) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * p.scale1);
-        }
         if (ROWS_M) {
-          float u[32];
+          // 32 rows x 128 bytes into a staging block in the 128-byte swizzle (16-byte piece c of row r at c ^ (r & 7):
+          // eight lanes touch eight bank groups), from there as whole lines to the output.
+          unsigned char *blk = blocks + (p.staging == 2 ? (nblk & 1) * kStageOut : 0);
+          ++nblk;
+          if (p.tma_store) {  // the block's last store has read it
+            if (lane == 0) {
+              if (p.staging == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+          }
           if (p.bias) {
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 bb = *reinterpret_cast<const float4 *>(bias_row + j);
-              u[j] = finish(v[j], p.scale, bb.x, p.relu); u[j + 1] = finish(v[j + 1], p.scale, bb.y, p.relu);
-              u[j + 2] = finish(v[j + 2], p.scale, bb.z, p.relu); u[j + 3] = finish(v[j + 3], p.scale, bb.w, p.relu);
+            for (int k = 0; k < kUnit; k += 32) bias_row[k + lane] = n + k + lane < p.n_extent ? p.bias[n + k + lane] : 0.f;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < kUnit / 32; ++h) {
+            tmem_ld32(acc + unit * kUnit + h * 32, v);
+            if (p.scale1 != 1.f) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * p.scale1);
+            }
+            constexpr int kPer = 16 / (int)sizeof(T);  // values of a 16-byte piece
+#pragma unroll
+            for (int j = 0; j < 32; j += kPer) {
+              alignas(16) T out[kPer];
+#pragma unroll
+              for (int k = 0; k < kPer; k += 4) {
+                float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.bias) bb = *reinterpret_cast<const float4 *>(bias_row + h * 32 + j + k);
+                out[k] = to_type<T>(finish(v[j + k], p.scale, bb.x, p.relu)); out[k + 1] = to_type<T>(finish(v[j + k + 1], p.scale, bb.y, p.relu));
+                out[k + 2] = to_type<T>(finish(v[j + k + 2], p.scale, bb.z, p.relu)); out[k + 3] = to_type<T>(finish(v[j + k + 3], p.scale, bb.w, p.relu));
+              }
+              const int piece = (h * 32 + j) / kPer;
+              *reinterpret_cast<uint4 *>(blk + lane * 128 + ((piece ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(out);
+            }
+          }
+          if (p.tma_store) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (mq < p.m_extent && n < p.n_extent) tma_store_2d(&map_y, smem_u32(blk), n, mq);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {
+            __syncwarp();
+            constexpr int kAside = 4 / (int)sizeof(T);  // values of a lane
+            const int left = p.n_extent - n - lane * kAside, rows = min(32, p.m_extent - mq);
+            T *y = static_cast<T *>(p.y) + (int64_t)mq * p.ld + n + lane * kAside;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r, y += p.ld) {
+              const T *from = reinterpret_cast<const T *>(blk + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = finish(v[j], p.scale, 0.f, p.relu);
+              for (int k = 0; k < kAside; ++k)
+                if (k < left) y[k] = from[k];
+            }
           }
-          if (m < p.m_extent) store_row<T>(static_cast<T *>(p.y) + (int64_t)m * p.ld + n, u, p.n_extent - n, p.vec);
         } else {
-          const int left = m < p.m_extent ? p.n_extent - n : 0;
-          T *y = static_cast<T *>(p.y) + (int64_t)n * p.ld + m;
+          tmem_ld32(acc + unit * 32, v);
+          if (p.scale1 != 1.f) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < left) y[j * p.ld] = to_type<T>(finish(v[j], p.scale, lane_bias, p.relu));
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * p.scale1);
+          }
+          const int rows = min(32, p.n_extent - n);
+          T *y = static_cast<T *>(p.y) + (int64_t)n * p.ld + m;
+          if (m < p.m_extent) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j, y += p.ld)
+              if (j < rows) *y = to_type<T>(finish(v[j], p.scale, lane_bias, p.relu));
+          }
         }
       }
+      if (t + tile_step < p.total_tiles) decode(p, t + tile_step, m0, n0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -439,35 +460,40 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         mbar_arrive(bar_pempty(b));
       }
     }
+    if (ROWS_M && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // this warp's stores are complete
   } else {
-    // The slices of a tile meet: a CTA owns 2^per_log columns; each pushes its sums of a column (128 lanes) to
-    // the owner, who adds them up in slice order.
-    const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;
+    // The slices of a tile meet: a CTA owns 2^per_log columns; each sends its sums of a column (128 lanes) to
+    // the owner, who adds them up in slice order.  They are laid out in the ring, which is idle, and leave as
+    // one copy per owner.
+    const int quarter = warp & 3, half = (warp - kFirstStore) >> 2, per = 1 << p.per_log;
     decode(p, tile0, m0, n0);
     const int live = min(p.nt, p.n_extent - n0);
-    bool ok = mbar_wait(bar_pfull(0), 0, abort_flag);
-    cluster_wait();  // (every CTA of the cluster runs)
-    ok = __all_sync(0xffffffffu, ok);
+    bool ok = __all_sync(0xffffffffu, mbar_wait(bar_pfull(0), 0, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (ok) {
-      const uint32_t mine = smem_u32(sums) + (uint32_t)(quarter * 32 + lane) * 4u, bar = bar_sums();
+    float *out = reinterpret_cast<float *>(ring);
 #pragma unroll 1
-      for (int c = half * 8; c < live; c += 16) {
-        uint32_t v[8];
-        tmem_ld8(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+    for (int c = half * 32; c < live; c += 64) {
+      uint32_t v[32];
+      tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int owner = (c + j) >> p.per_log, at = (rank << p.per_log) + (c + j - (owner << p.per_log));
-          if (c + j < live) st_async(cluster_addr(mine + (uint32_t)(at * kSumPitch) * 4u, owner), v[j], cluster_addr(bar, owner));
-        }
-      }
+      for (int j = 0; j < 32; ++j)
+        if (c + j < live) out[(c + j) * kSumPitch + quarter * 32 + lane] = __uint_as_float(v[j]);
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    cluster_wait();  // (every CTA of the cluster runs)
+    asm volatile("bar.sync 1, %0;" ::"r"(32 * kStoreWarps) : "memory");
+    if (warp == kFirstStore && lane < p.d && ok && !*abort_flag) {
+      const int cols = min(per, live - (lane << p.per_log));
+      if (cols > 0)
+        push(cluster_addr(smem_u32(sums) + (uint32_t)((rank << p.per_log) * kSumPitch) * 4u, lane), smem_u32(out) + (uint32_t)((lane << p.per_log) * kSumPitch) * 4u,
+             (uint32_t)(cols * kSumPitch) * 4u, cluster_addr(bar_sums(), lane));
+    }
+    __syncwarp();
     ok = __all_sync(0xffffffffu, mbar_wait(bar_sums(), 0, abort_flag)) && ok;
-    cluster_arrive();  // (what this CTA is owed has come, or it has given up; all of its own pushes are on their way)
-    const int own = ok ? min(1 << p.per_log, live - (rank << p.per_log)) : 0, own0 = n0 + (rank << p.per_log);
-    const int e0 = tid - 32 * kFirstStore;
+    cluster_arrive();  // (what this CTA is owed has come, or it has given up; all of its own copies have been sent)
+    const int own = ok ? min(per, live - (rank << p.per_log)) : 0, own0 = n0 + (rank << p.per_log);
     // D[oc][row]: neighbouring threads take neighbouring lanes; D[row][oc]: neighbouring columns
-    for (int e = e0; e < own * kM; e += 32 * kStoreWarps) {
+    for (int e = tid - 32 * kFirstStore; e < own * kM; e += 32 * kStoreWarps) {
       const int j = ROWS_M ? e % own : e / kM, l = ROWS_M ? e / own : e % kM;
       if (m0 + l >= p.m_extent) continue;
       float u = 0.f;
@@ -545,7 +571,7 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
 }
 
 template <int FMT, typename T, bool ROWS_M>
-int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
+int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
   static bool ready[64] = {};  // per device
   int dev = 0;
   TETRIS_CUDA_TRY(cudaGetDevice(&dev));
@@ -553,21 +579,22 @@ int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const ProductPara
     TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024)));
     if (dev < 64) ready[dev] = true;
   }
-  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, p));
+  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, map_y, p));
   count_launch();
   return TETRIS_OK;
 }
 template <int FMT, typename T>
-int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
-  return rows_m ? launch<FMT, T, true>(map_m, map_n, p, grid, smem, st) : launch<FMT, T, false>(map_m, map_n, p, grid, smem, st);
+int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
+  return rows_m ? launch<FMT, T, true>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false>(map_m, map_n, map_y, p, grid, smem, st);
 }
 
-int encode(CUtensorMap *map, const uint8_t *codes, int64_t pitch, int64_t rows, int box_rows) {
+// A matrix whose rows are `pitch` bytes apart, in boxes of 128 bytes x `box_rows`.
+int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const void *matrix, int64_t cols, int64_t pitch, int64_t rows, int box_rows) {
   EncodeFn enc = get_encode();
   if (!enc) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return TETRIS_ERR_UNSUPPORTED; }
-  const cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, one[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {128u / (cuuint32_t)type_bytes, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const CUresult r = enc(map, type, 2, const_cast<void *>(matrix), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with code %d", (int)r); return TETRIS_ERR_CUDA; }
   return TETRIS_OK;
@@ -594,6 +621,8 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
   p.m_tiles = p.m_blocks;
   p.n_tiles = (p.n_extent + g.nt - 1) / g.nt;
   p.group = std::min(p.m_tiles, 16);
+  p.by_per = fp4_div((uint32_t)(p.group * p.n_tiles)); p.by_group = fp4_div((uint32_t)p.group);
+  p.by_last = fp4_div((uint32_t)std::max(1, p.m_tiles % p.group));
   const int64_t total = (int64_t)p.m_tiles * p.n_tiles;
   if (total > 0x3FFFFFFF) { set_error("a product of %lld tiles is outside what the kernels cover", (long long)total); return TETRIS_ERR_UNSUPPORTED; }
   p.total_tiles = (int)total;
@@ -601,7 +630,8 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
   p.sm_at = p.n_at + g.nt * 128;
   p.sn_at = p.sm_at + kt * 512;
   p.stage_bytes = (p.sn_at + rt * kt * 512 + 1023) / 1024 * 1024;
-  const size_t tail = (g.d > 1 ? (size_t)g.nt * kSumPitch * 4 : 0) + kBiasBytes + kBars * 8 + 16;
+  p.staging = !g.rows_m ? 0 : rt == 2 ? 1 : 2;
+  const size_t tail = (g.d > 1 ? (size_t)g.nt * kSumPitch * 4 : (size_t)kStoreWarps * kStageOut * p.staging) + kBiasBytes + kBars * 8 + 16;
   p.stages = std::min<int>(kStagesMax, (int)((kSmemMost - tail) / p.stage_bytes));
   p.slot_cols = 4 * kt * (1 + rt);
   p.slots = rt == 2 ? 2 : std::min(kSlotsMax, p.stages);  // (at most `stages`: a step's empty barrier is waited for before the stage is used again)
@@ -610,20 +640,24 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
   const int e = exponent + f->exponent, e0 = std::max(-126, std::min(126, e));
   p.scale = ldexpf(1.f, e0); p.scale1 = ldexpf(1.f, e - e0);
   p.relu = relu;
-  for (p.vec = 32; p.vec >= 16 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes)) & (p.vec - 1)); p.vec /= 2) {}
-  if (p.vec < 16) p.vec = 0;
+  // (the distance between rows in a tensor map is below 2^40 bytes)
+  p.tma_store = g.rows_m && g.d == 1 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes)) & 15) == 0 && ld * bytes < (1ll << 40);
   p.error_flag = f->d_error;
   p.withhold_first_load = test_injection(&p.spin_limit);
-  CUtensorMap map_w, map_a;
+  CUtensorMap map_w, map_a, map_y = {};
   int rc;
-  if ((rc = encode(&map_w, f->d_codes, f->pitch, f->out_channel, g.rows_m ? g.nt : kM)) || (rc = encode(&map_a, codes, f->pitch, rows, g.rows_m ? kM : g.nt))) return rc;
+  if ((rc = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, f->d_codes, f->pitch, f->pitch, f->out_channel, g.rows_m ? g.nt : kM)) ||
+      (rc = encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, f->pitch, f->pitch, rows, g.rows_m ? kM : g.nt)) ||
+      (p.tma_store && (rc = encode(&map_y, y_type == TETRIS_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, bytes, y,
+                                   f->out_channel, ld * bytes, rows, 32))))
+    return rc;
   const CUtensorMap &map_m = g.rows_m ? map_a : map_w, &map_n = g.rows_m ? map_w : map_a;
   const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, f->sm_count));
   const size_t smem = std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail + 1024);
   switch (y_type) {
-    case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, p, grid, smem, st);
-    case TETRIS_BF16: return nv ? launch<TETRIS_FP4_NV, __nv_bfloat16>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, __nv_bfloat16>(g.rows_m, map_m, map_n, p, grid, smem, st);
-    default: return nv ? launch<TETRIS_FP4_NV, __half>(g.rows_m, map_m, map_n, p, grid, smem, st) : launch<TETRIS_FP4_MX, __half>(g.rows_m, map_m, map_n, p, grid, smem, st);
+    case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
+    case TETRIS_BF16: return nv ? launch<TETRIS_FP4_NV, __nv_bfloat16>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, __nv_bfloat16>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
+    default: return nv ? launch<TETRIS_FP4_NV, __half>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, __half>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
   }
 }
 
