@@ -157,8 +157,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
                : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// (whole warps, whatever a role's lanes did before)
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {  // `addr` of this CTA in CTA `rank` of the cluster
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -492,15 +499,35 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     ok = __all_sync(0xffffffffu, mbar_wait(bar_sums(), 0, abort_flag)) && ok;
     cluster_arrive();  // (what this CTA is owed has come, or it has given up; all of its own copies have been sent)
     const int own = ok ? min(per, live - (rank << p.per_log)) : 0, own0 = n0 + (rank << p.per_log);
-    // D[oc][row]: neighbouring threads take neighbouring lanes; D[row][oc]: neighbouring columns
-    for (int e = tid - 32 * kFirstStore; e < own * kM; e += 32 * kStoreWarps) {
-      const int j = ROWS_M ? e % own : e / kM, l = ROWS_M ? e / own : e % kM;
-      if (m0 + l >= p.m_extent) continue;
-      float u = 0.f;
-      for (int s = 0; s < p.d; ++s) u += sums[((s << p.per_log) + j) * kSumPitch + l];
-      const int row = ROWS_M ? m0 + l : own0 + j, oc = ROWS_M ? own0 + j : m0 + l;
-      u = finish(__float_as_uint(u * p.scale1), p.scale, p.bias ? p.bias[oc] : 0.f, p.relu);
-      static_cast<T *>(p.y)[(int64_t)row * p.ld + oc] = to_type<T>(u);
+    // A thread takes four lanes of a column.  D[oc][row]: neighbouring threads take neighbouring lanes; D[row][oc]:
+    // neighbouring columns.
+    const bool whole = !ROWS_M && ((reinterpret_cast<uintptr_t>(p.y) | (uint64_t)(p.ld * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+    for (int e = tid - 32 * kFirstStore; e < per * (kM / 4); e += 32 * kStoreWarps) {
+      const int j = ROWS_M ? e & (per - 1) : e / (kM / 4), l = 4 * (ROWS_M ? e >> p.per_log : e % (kM / 4));
+      if (j >= own || m0 + l >= p.m_extent) continue;
+      const float *from = sums + j * kSumPitch + l;
+      float u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int s = 0; s < p.d; ++s) {
+        const float4 a = *reinterpret_cast<const float4 *>(from + (s << p.per_log) * kSumPitch);
+        u[0] += a.x; u[1] += a.y; u[2] += a.z; u[3] += a.w;
+      }
+      T *y = static_cast<T *>(p.y) + (ROWS_M ? (int64_t)(m0 + l) * p.ld + own0 + j : (int64_t)(own0 + j) * p.ld + m0 + l);
+      alignas(16) T out[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int oc = ROWS_M ? own0 + j : m0 + l + k;
+        const float bias = p.bias && (ROWS_M || oc < p.m_extent) ? p.bias[oc] : 0.f;
+        out[k] = to_type<T>(finish(__float_as_uint(u[k] * p.scale1), p.scale, bias, p.relu));
+      }
+      if (whole && m0 + l + 4 <= p.m_extent) {
+        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(out);
+        else *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(out);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m0 + l + k < p.m_extent) y[ROWS_M ? k * p.ld : k] = out[k];
+      }
     }
   }
   __syncwarp();
