@@ -38,7 +38,6 @@ constexpr int kStoreWarps = 8, kFirstStore = 2, kThreads = 32 * (kFirstStore + k
 constexpr int kStagesMax = 8, kSlotsMax = 8;
 constexpr int kBars = 2 * kStagesMax + 8;
 constexpr uint32_t kSpinLimit = 1u << 22;
-constexpr int kTmemCols = 512;
 constexpr int kSumPitch = kM + 4;        // floats between the columns of a cluster's sums (whole 16 bytes)
 constexpr int kBiasBytes = kStoreWarps * 64 * 4;
 constexpr int kStageOut = 4096;          // a staging block: 32 rows of 128 bytes on their way to the output
@@ -61,7 +60,8 @@ struct ProductParams {
   int d, per_log;          // CTAs of a cluster = slices of a tile's K range; log2 of the columns a CTA owns
   int stages, slots;
   int stage_bytes, n_at, sm_at, sn_at;  // a stage: codes of M and N, scales of M and N
-  int acc1, sf, slot_cols; // columns of the second accumulator, the scales, of a slot of them
+  int tmem_cols;
+  int accs, acc1, sf, slot_cols; // accumulators; columns of the second one, the scales, of a slot of them
   float scale, scale1;     // 2^(sum of the exponents), as two factors where one would leave FP32
   int relu;
   int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows)
@@ -200,7 +200,7 @@ __device__ __forceinline__ float finish(uint32_t v, float scale, float bias, int
 }
 
 template <int FMT, typename T, bool ROWS_M>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
 product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const __grid_constant__ CUtensorMap map_y,
                const ProductParams p) {
   constexpr int kTiles = step_tiles(FMT);
@@ -226,7 +226,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   const int tile0 = p.d > 1 ? blockIdx.x / p.d : blockIdx.x, tile_step = p.d > 1 ? gridDim.x / p.d : gridDim.x;
   const int step0 = p.d > 1 ? (int)((int64_t)p.steps * rank / p.d) : 0, step1 = p.d > 1 ? (int)((int64_t)p.steps * (rank + 1) / p.d) : p.steps;
   const int rt = p.nt > 128 ? 2 : 1;       // 128-row blocks of a tile's N scales
-  const bool over = p.acc1 < p.nt;         // the accumulators share columns
+  const bool over = p.accs == 2 && p.acc1 < p.nt;  // the accumulators share columns
+  const int acc_log = p.accs - 1;          // tile i uses accumulator i & acc_log, for the (i >> acc_log)-th time
   const int ahead = min(step1 - step0, p.stages);
   int loads = 0;
   int m0, n0;
@@ -273,7 +274,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     }
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(p.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -313,10 +314,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     int i = 0;
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
       decode(p, t, m0, n0);
-      const int b = i & 1;
+      const int b = i & acc_log;
       const uint32_t acc = tmem + (b ? p.acc1 : 0);
       const uint32_t sf_row = (uint32_t)(n0 & 127) >> 5;   // the tile's first 32-row group within its scale tile: 0 or 2
-      if (i >= 2) wait(bar_pempty(b), ((i >> 1) & 1) ^ 1);
+      if (i > acc_log) wait(bar_pempty(b), ((i >> acc_log) & 1) ^ 1);
       if (over && i >= 1) wait(bar_shared(b ^ 1), ((i - 1) >> 1) & 1);
       for (int step = step0; step < step1; ++step) {
         if (behind == p.slots) {
@@ -367,9 +368,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     int i = 0;
     decode(p, tile0, m0, n0);
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
-      const int b = i & 1, mq = m0 + quarter * 32, m = mq + lane, n_first = n0;
+      const int b = i & acc_log, mq = m0 + quarter * 32, m = mq + lane, n_first = n0;
       const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
-      if (!mbar_try_wait(bar_pfull(b), (i >> 1) & 1)) mbar_wait(bar_pfull(b), (i >> 1) & 1, abort_flag);
+      if (!mbar_try_wait(bar_pfull(b), (i >> acc_log) & 1)) mbar_wait(bar_pfull(b), (i >> acc_log) & 1, abort_flag);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (b ? p.acc1 : 0);
@@ -550,7 +551,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     __syncwarp();
   }
   if (p.d > 1) cluster_wait();  // (no CTA leaves while another one may still push into it)
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -564,19 +565,24 @@ EncodeFn get_encode() {
   return fn;
 }
 
-constexpr size_t kSmemMost = 227 * 1024 - 1024;   // (the ring is aligned to 1024 bytes)
-constexpr size_t kSmemLeast = 117 * 1024;         // one CTA per SM, also beside the other kernels that take all of an SM's tensor memory
+// A product takes half of an SM (113 KB of shared memory, 256 columns of tensor memory) or all of it.  Two halves
+// overlap: one CTA stores while the other one computes, and the next launch is placed and fetches its filter while
+// this one ends.  Nothing that holds tensor memory and waits for another CTA may sit beside a CTA that waits for
+// tensor memory: two halves always fit, and a half beside anything that takes 116 KB or more never does.
+constexpr size_t kSmemMost = 227 * 1024, kSmemHalf = 113 * 1024;   // (1 KB of either goes into the ring's alignment)
+constexpr size_t kSmemLeast = 117 * 1024;
 
 struct Geometry {
   bool rows_m;
   int nt, d;
+  bool half;
 };
 
 // The least of an estimate in clocks: waves of tiles, each K step at the longer of its MMAs and its loads
 // (about 44 bytes a clock and SM from L2), the store of the last tile, the meeting of a cluster.
 Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
   const int steps = (f->in_channel + kStep - 1) / kStep;
-  Geometry best = {false, 16, 1};
+  Geometry best = {false, 16, 1, true};
   double least = 1e300;
   for (int rows_m = 0; rows_m < 2; ++rows_m) {
     const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
@@ -590,7 +596,7 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
         const double waves = (double)((tiles * d + f->sm_count - 1) / f->sm_count);
         const double step = std::max(2.0 * nt, (kM + nt) * 144 / 44.0), store = (rows_m ? 4.0 : 8.0) * nt;
         const double cost = waves * std::max((double)((steps + d - 1) / d) * step, store) + (d > 1 ? 1500 + 4.0 * nt : store);
-        if (cost < least) { least = cost; best = {rows_m != 0, nt, d}; }
+        if (cost < least) { least = cost; best = {rows_m != 0, nt, d, nt <= 64 || (nt == 128 && d == 1)}; }
       }
     }
   }
@@ -603,7 +609,7 @@ int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap
   int dev = 0;
   TETRIS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024)));
+    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost));
     if (dev < 64) ready[dev] = true;
   }
   TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, map_y, p));
@@ -657,13 +663,15 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
   p.sm_at = p.n_at + g.nt * 128;
   p.sn_at = p.sm_at + kt * 512;
   p.stage_bytes = (p.sn_at + rt * kt * 512 + 1023) / 1024 * 1024;
-  p.staging = !g.rows_m ? 0 : rt == 2 ? 1 : 2;
-  const size_t tail = (g.d > 1 ? (size_t)g.nt * kSumPitch * 4 : (size_t)kStoreWarps * kStageOut * p.staging) + kBiasBytes + kBars * 8 + 16;
-  p.stages = std::min<int>(kStagesMax, (int)((kSmemMost - tail) / p.stage_bytes));
+  p.staging = !g.rows_m ? 0 : rt == 2 || g.half ? 1 : 2;
+  const size_t tail = 1024 + (g.d > 1 ? (size_t)g.nt * kSumPitch * 4 : (size_t)kStoreWarps * kStageOut * p.staging) + kBiasBytes + kBars * 8 + 16;
+  p.stages = std::min<int>(kStagesMax, (int)(((g.half ? kSmemHalf : kSmemMost) - tail) / p.stage_bytes));
+  p.tmem_cols = g.half ? 256 : 512;
   p.slot_cols = 4 * kt * (1 + rt);
-  p.slots = rt == 2 ? 2 : std::min(kSlotsMax, p.stages);  // (at most `stages`: a step's empty barrier is waited for before the stage is used again)
-  p.sf = kTmemCols - p.slots * p.slot_cols;
-  p.acc1 = std::min(std::max(g.nt, 32), (p.sf - g.nt) / 32 * 32);
+  p.accs = g.half && g.nt > 64 ? 1 : 2;
+  p.slots = rt == 2 ? 2 : std::min(g.half ? 4 : kSlotsMax, p.stages);  // (at most `stages`: a step's empty barrier is waited for before the stage is used again)
+  p.sf = p.tmem_cols - p.slots * p.slot_cols;
+  p.acc1 = p.accs == 2 ? std::min(std::max(g.nt, 32), (p.sf - g.nt) / 32 * 32) : 0;
   const int e = exponent + f->exponent, e0 = std::max(-126, std::min(126, e));
   p.scale = ldexpf(1.f, e0); p.scale1 = ldexpf(1.f, e - e0);
   p.relu = relu;
@@ -679,8 +687,8 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
                                    f->out_channel, ld * bytes, rows, 32))))
     return rc;
   const CUtensorMap &map_m = g.rows_m ? map_a : map_w, &map_n = g.rows_m ? map_w : map_a;
-  const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, f->sm_count));
-  const size_t smem = std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail + 1024);
+  const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, (g.half ? 2 : 1) * f->sm_count));
+  const size_t smem = g.half ? kSmemHalf : std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail);
   switch (y_type) {
     case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
     case TETRIS_BF16: return nv ? launch<TETRIS_FP4_NV, __nv_bfloat16>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, __nv_bfloat16>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
