@@ -511,3 +511,29 @@ def test_refusals_on_the_device(tb, torch_cuda):
     tb.fp4_conv2d(f, x[:0], y[:0], 0, 10, 10, 1, 0, work)
     torch.cuda.synchronize()
     assert bool((y == 5.0).all())
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
+def test_bounded_wait_gives_up_and_the_next_product_passes(tb, torch_cuda, rows):
+    """Every CTA leaves out its first activations: the waits run out, the launch returns, the status is read, and
+    the next product of the same filter is right."""
+    torch = torch_cuda
+    k, n = 600, 200
+    f, w = filter_and_weights(tb, torch, n, k, ref.NV, 31)
+    x = activations(torch, rows, k, 32, spread=1.0)
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    y = torch.empty(rows, n, device="cuda")
+    torch.cuda.synchronize()
+    tb.test_inject(1, 2000)
+    try:
+        tb.fp4_linear(f, x, y, rows, work)
+        with pytest.raises(tb.TetrisError) as e:
+            f.check()
+        assert e.value.status == 2 and "gave up" in str(e.value)
+    finally:
+        tb.test_inject(0)
+    f.check()
+    tb.fp4_linear(f, x, y, rows, work)
+    f.check()
+    want, terms = reference_product(x, w, ref.NV, 0, f.exponent_)
+    check_product(y, want, terms, k, torch)

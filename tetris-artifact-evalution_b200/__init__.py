@@ -443,7 +443,7 @@ _fp4_type_of = {}                 # torch dtype -> type, filled as dtypes are me
 
 def _fp4_type(x, dtype, what):
     """The type of a dense argument: `dtype` for an address, the tensor's own for a tensor."""
-    if isinstance(x, int):
+    if type(x) is int:
         return FP32 if dtype is None else dtype
     t = _fp4_type_of.get(x.dtype)
     if t is None:
@@ -459,18 +459,17 @@ def _fp4_type(x, dtype, what):
 def _fp4_dense(x, rows, cols, ld, what):
     """(address, row distance) of a dense device matrix of rows x cols.  A two-dimensional tensor may have
     rows further apart than cols; any other has to be contiguous."""
-    if isinstance(x, int):
+    if type(x) is int:
         return x, ld
-    if x.dim() == 2 and x.shape[0] == rows and x.shape[1] == cols:
-        if rows > 1 or cols > 1:
-            apart, step = x.stride()
-            if (step != 1 and cols > 1) or (apart < cols and rows > 1):
-                raise ValueError("the columns of %s have to lie side by side, its strides are %s" % (what, tuple(x.stride())))
-            if ld and rows > 1 and ld != apart:
-                raise ValueError("rows of %s lie %d elements apart, %d was named" % (what, apart, ld))
-            if rows > 1:
-                return x.data_ptr(), apart
+    if not ld and x.is_contiguous() and x.numel() == rows * cols:
         return x.data_ptr(), 0
+    if x.dim() == 2 and x.shape[0] == rows and x.shape[1] == cols:
+        apart, step = x.stride()
+        if (step != 1 and cols > 1) or (apart < cols and rows > 1):
+            raise ValueError("the columns of %s have to lie side by side, its strides are %s" % (what, tuple(x.stride())))
+        if ld and rows > 1 and ld != apart:
+            raise ValueError("rows of %s lie %d elements apart, %d was named" % (what, apart, ld))
+        return x.data_ptr(), apart if rows > 1 else 0
     if not x.is_contiguous():
         raise ValueError("%s is neither a %d x %d matrix nor contiguous" % (what, rows, cols))
     need = (rows - 1) * (ld or cols) + cols if rows else 0
@@ -481,15 +480,15 @@ def _fp4_dense(x, rows, cols, ld, what):
 
 def _fp4_bytes(x, need, what):
     """Address of a device buffer of at least `need` bytes."""
-    if isinstance(x, int):
+    if type(x) is int:
         return x
-    if not x.is_contiguous() or x.numel() * x.element_size() < need:
+    if not x.is_contiguous() or x.nbytes < need:
         raise ValueError("%s has to be contiguous and hold %d bytes" % (what, need))
     return x.data_ptr()
 
 
 def _fp4_bias(bias, out_channel):
-    if bias is None or isinstance(bias, int):
+    if bias is None or type(bias) is int:
         return bias
     if _fp4_type(bias, None, "bias") != FP32 or not bias.is_contiguous() or bias.numel() < out_channel:
         raise ValueError("the bias has to be %d contiguous float32 values" % out_channel)
@@ -613,11 +612,11 @@ def _fp4_room(workspace):
     """(address, bytes) of a workspace; an address is taken to be large enough."""
     if workspace is None:
         return None, 0
-    if isinstance(workspace, int):
+    if type(workspace) is int:
         return workspace, 1 << 62
     if not workspace.is_contiguous():
         raise ValueError("the workspace has to be contiguous")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def fp4_linear(fp4_filter, input, output, rows, workspace=None, exponent=0, bias=None, relu=False, ld_input=0, ld_output=0,
@@ -625,12 +624,16 @@ def fp4_linear(fp4_filter, input, output, rows, workspace=None, exponent=0, bias
     """`output` (rows x out_channel) = `input` (rows x in_channel, FP32 / BF16 / FP16), quantised on the way,
     times the filter (+ bias, ReLU), asynchronous.  `workspace`: fp4_workspace bytes on the device."""
     f = fp4_filter
+    n = f.out_channel_
     x, ld_input = _fp4_dense(input, rows, f.in_channel_, ld_input, "the input")
-    y, ld_output = _fp4_dense(output, rows, f.out_channel_, ld_output, "the output")
-    room = _fp4_room(workspace)
-    _check(lib().tetris_fp4_linear(f.handle, x, _fp4_type(input, input_dtype, "the input"), rows, ld_input, exponent,
-                                   _fp4_bias(bias, f.out_channel_), y, _fp4_type(output, output_dtype, "the output"), ld_output,
-                                   FUSE_RELU if relu else 0, room[0], room[1], _stream_ptr(cuda_stream)))
+    y, ld_output = _fp4_dense(output, rows, n, ld_output, "the output")
+    room, size = _fp4_room(workspace)
+    status = lib().tetris_fp4_linear(f.handle, x, _fp4_type(input, input_dtype, "the input"), rows, ld_input, exponent,
+                                     None if bias is None else _fp4_bias(bias, n), y,
+                                     _fp4_type(output, output_dtype, "the output"), ld_output, FUSE_RELU if relu else 0, room, size,
+                                     None if cuda_stream is None else _stream_ptr(cuda_stream))
+    if status:
+        _check(status)
 
 
 def fp4_conv2d(fp4_filter, input, output, batch_size, img_h, img_w, stride, padding, workspace=None, exponent=0, bias=None,

@@ -2,6 +2,7 @@
 // and fp4_product.cu share.  The formats and their storage are described in the public header.
 #pragma once
 #include <cuda.h>
+#include <math.h>
 
 #include "internal.h"
 
@@ -35,6 +36,13 @@ inline int64_t fp4_pitch(int cols) { return ((int64_t)cols + 31) / 32 * 16; }
 inline int fp4_tiles(int cols, int format) { return (int)(((int64_t)cols + 4 * fp4_block(format) - 1) / (4 * fp4_block(format))); }
 inline int64_t fp4_scale_bytes(int64_t rows, int cols, int format) { return (rows + 127) / 128 * fp4_tiles(cols, format) * 512; }
 
+// 2^exponent, 1 / (6 * 2^exponent) and what its rounding left.
+inline void fp4_scale_factors(int exponent, float *tensor_scale, float *sixth, float *sixth_rest) {
+  *tensor_scale = ldexpf(1.f, exponent);
+  *sixth = ldexpf(1.f / 6.f, -exponent);
+  *sixth_rest = (float)ldexp(1.0 / 6.0 - (double)(1.f / 6.f), -exponent);
+}
+
 // Rows of a quantisation that are pixels of a strided layer: row (n, oh, ow) reads pixel (n, oh * S, ow * S).
 struct Fp4Pixels {
   int H, W, OH, OW, S;
@@ -49,7 +57,15 @@ int launch_fp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t r
 int launch_fp4_largest(const void *x, int x_type, int64_t n, unsigned *d_bits, cudaStream_t st);
 
 // fp4_product.cu
-int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const uint8_t *scales, int64_t rows, int exponent, const float *bias,
-                       void *y, int y_type, int64_t ld, int relu, cudaStream_t st);
+struct Fp4Rows {             // activations of a product
+  const uint8_t *codes, *scales;  // quantised ...
+  const void *x;             // ... or, where codes is null, as they are: at most kFp4DirectRows rows
+  int x_type;
+  int64_t ld;
+  const Fp4Pixels *px;
+};
+constexpr int kFp4DirectRows = 4;  // up to here a product quantises its activations itself
+int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
+                       int relu, cudaStream_t st);
 
 }  // namespace tetris

@@ -62,7 +62,7 @@ int check_filter(const tetris_fp4_filter *f) {
 
 int64_t workspace_codes(const tetris_fp4_filter *f, int64_t rows) { return (rows * f->pitch + 255) / 256 * 256; }
 int64_t workspace_bytes(const tetris_fp4_filter *f, int64_t rows) {
-  return rows == 0 ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
+  return rows <= kFp4DirectRows ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
 }
 
 // Checks that all products share; the filter's device is current.
@@ -88,9 +88,10 @@ int linear(const tetris_fp4_filter *f, const void *x, int x_type, int64_t rows, 
   const int64_t need = workspace_bytes(f, rows);
   if (bytes < need) { set_error("a workspace of %lld bytes, %lld are needed", (long long)bytes, (long long)need); return TETRIS_ERR_INVALID; }
   if (need && (rc = check_memory("workspace", workspace, f->device, 16))) return rc;
+  if (!need) return launch_fp4_product(f, {nullptr, nullptr, x, x_type, ld_x, px}, rows, exponent, bias, y, y_type, ld_y, flags & TETRIS_FUSE_RELU, st);
   uint8_t *codes = static_cast<uint8_t *>(workspace), *scales = codes + workspace_codes(f, rows);
   if ((rc = launch_fp4_quantize(x, x_type, rows, f->in_channel, ld_x, px, f->format, exponent, codes, scales, st))) return rc;
-  return launch_fp4_product(f, codes, scales, rows, exponent, bias, y, y_type, ld_y, flags & TETRIS_FUSE_RELU, st);
+  return launch_fp4_product(f, {codes, scales, nullptr, 0, 0, nullptr}, rows, exponent, bias, y, y_type, ld_y, flags & TETRIS_FUSE_RELU, st);
 }
 
 }  // namespace
@@ -280,8 +281,8 @@ int tetris_fp4_product(const tetris_fp4_filter_t *f, const void *d_codes, const 
   DeviceGuard guard(f->device);
   if ((rc = check_product(f, rows, exponent, d_bias, d_y, y_type, &ld, flags)) || rows == 0) return rc;
   if ((rc = check_memory("codes", d_codes, f->device, 16)) || (rc = check_memory("scales", d_scales, f->device, 16))) return rc;
-  return launch_fp4_product(f, static_cast<const uint8_t *>(d_codes), static_cast<const uint8_t *>(d_scales), rows, exponent, d_bias, d_y, y_type,
-                            ld, flags & TETRIS_FUSE_RELU, (cudaStream_t)stream);
+  return launch_fp4_product(f, {static_cast<const uint8_t *>(d_codes), static_cast<const uint8_t *>(d_scales), nullptr, 0, 0, nullptr}, rows, exponent,
+                            d_bias, d_y, y_type, ld, flags & TETRIS_FUSE_RELU, (cudaStream_t)stream);
 }
 
 int tetris_fp4_workspace(const tetris_fp4_filter_t *f, int64_t rows, int64_t *bytes) {

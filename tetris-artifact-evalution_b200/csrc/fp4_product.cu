@@ -13,6 +13,8 @@
 //     zeros past both ends) and bulk copies of the scales, into one ring;
 //   * warp 1 (one elected lane): scales from shared into tensor memory (tcgen05.cp), then 4 MMAs;
 //   * eight storing warps: accumulator -> scale, bias, ReLU -> output, beside the next tile's MMAs.
+// Up to 4 rows that are not quantised yet: the storing warps first turn them into codes and scales in shared
+// memory, a row's 256 values of a K step per warp, while the filter is on its way.
 // Tensor memory: two accumulators.  With N = 256 two of them and the scales exceed 512 columns, so the
 // second one lies over the end of the first; the storing warps empty the shared columns first and the next
 // tile starts once those are free.
@@ -28,6 +30,7 @@
 #include <algorithm>
 
 #include "fp4.h"
+#include "fp4_block.h"
 
 namespace tetris {
 namespace {
@@ -63,6 +66,11 @@ struct ProductParams {
   int tmem_cols;
   int accs, acc1, sf, slot_cols; // accumulators; columns of the second one, the scales, of a slot of them
   float scale, scale1;     // 2^(sum of the exponents), as two factors where one would leave FP32
+  const void *x;           // activations that are not quantised yet
+  int x_type, x_vec, K;
+  int64_t x_ld;
+  Fp4Pixels px;            // (S > 1: a row is a pixel of a strided layer)
+  float tensor_scale, sixth, sixth_rest;  // as in the quantisation
   int relu;
   int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows)
   int staging;             // ... staging blocks of a storing warp: 1 or 2
@@ -199,7 +207,37 @@ __device__ __forceinline__ float finish(uint32_t v, float scale, float bias, int
   return u;
 }
 
-template <int FMT, typename T, bool ROWS_M>
+// 8 neighbouring values of a row, zeros behind the last one.
+__device__ __forceinline__ void load8(const ProductParams &p, int64_t at, int left, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  if (p.x_type == TETRIS_FP32) {
+    const float *x = static_cast<const float *>(p.x) + at;
+    if (p.x_vec && left >= 8) {
+      *reinterpret_cast<float4 *>(v) = reinterpret_cast<const float4 *>(x)[0];
+      *reinterpret_cast<float4 *>(v + 4) = reinterpret_cast<const float4 *>(x)[1];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < left) v[k] = x[k];
+    }
+    return;
+  }
+  const uint16_t *x = static_cast<const uint16_t *>(p.x) + at;
+  alignas(16) uint16_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (p.x_vec && left >= 8) {
+    *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(x);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left) h[k] = x[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = p.x_type == TETRIS_BF16 ? __uint_as_float((uint32_t)h[k] << 16) : __half2float(__ushort_as_half(h[k]));
+}
+
+// DIRECT: the rows (on the N side, at most kFp4DirectRows) are quantised here.
+template <int FMT, typename T, bool ROWS_M, bool DIRECT>
 __global__ void __launch_bounds__(kThreads, 2)
 product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const __grid_constant__ CUtensorMap map_y,
                const ProductParams p) {
@@ -247,17 +285,19 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   };
   auto load_filter = [&](int s, int step) {
     const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-    mbar_expect_tx(bar, (uint32_t)((kM + p.nt) * 128 + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
+    mbar_expect_tx(bar, DIRECT ? (uint32_t)(kM * 128 + scale_tiles(step) * 512)
+                               : (uint32_t)((kM + p.nt) * 128 + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
     if (ROWS_M) load_n(at, bar, step); else load_m(at, bar, step);
   };
   auto load_rows = [&](int s, int step) {
     const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
     if (loads++ == 0 && p.withhold_first_load) return;  // (test: that step never arrives, its reader gives up)
+    if (DIRECT) return;
     if (ROWS_M) load_m(at, bar, step); else load_n(at, bar, step);
   };
 
   if (tid == 0) {
-    for (int s = 0; s < kStagesMax; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < kStagesMax; ++s) { mbar_init(bar_full(s), DIRECT ? 1 + p.n_extent : 1); mbar_init(bar_empty(s), 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(bar_pfull(b), 1); mbar_init(bar_pempty(b), kStoreWarps); mbar_init(bar_shared(b), kStoreWarps); }
     mbar_init(bar_drain(), 1);
     mbar_init(bar_sums(), 1);
@@ -358,6 +398,56 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         if (++slot == p.slots) slot = 0;
       }
     }
+  }
+  if (DIRECT && warp >= kFirstStore) {
+    // Unit u: row u & (2^rows_log - 1) of K step u >> rows_log; warp w takes units w, w + 8, ..., a lane 8 values.
+    // Every warp walks all steps and waits for each stage that is used again: a wait for a barrier's phase by its parity
+    // only means something to who has seen the phase before.
+    constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8;
+    const int rows_log = p.n_extent > 2 ? 2 : p.n_extent - 1, units = (step1 - step0) << rows_log;
+    int u = warp - kFirstStore, s = 0;
+    uint32_t parity = 1;
+    float v[8];
+    auto fetch = [&]() {  // the values of unit u
+      const int step = step0 + (u >> rows_log), row = u & ((1 << rows_log) - 1), col = step * kStep + lane * 8;
+      int64_t from = row;
+      if (p.px.S > 1) {
+        const int y = row / p.px.OW, n = y / p.px.OH;
+        from = ((int64_t)n * p.px.H + (int64_t)(y - n * p.px.OH) * p.px.S) * p.px.W + (int64_t)(row - y * p.px.OW) * p.px.S;
+      }
+      load8(p, from * p.x_ld + col, u < units && row < p.n_extent ? p.K - col : 0, v);
+    };
+    fetch();
+#pragma unroll 1
+    for (int step = step0; step < step1; ++step) {
+      if (step - step0 >= p.stages) mbar_wait(bar_empty(s), parity, abort_flag);
+      if (u >> rows_log == step - step0) {
+        const int row = u & ((1 << rows_log) - 1);
+        if (row < p.n_extent) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);  // (as integers: NaN last)
+          __syncwarp();
+#pragma unroll
+          for (int l = 1; l < kLanes; l *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, l));
+          const uint8_t byte = scale_block<FMT>(v, __uint_as_float(top), p.tensor_scale, p.sixth, p.sixth_rest);
+          const int left = p.K - step * kStep - lane * 8;
+          const uint32_t codes = codes_of(v) & (left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u);
+          unsigned char *at = ring + (size_t)s * p.stage_bytes;
+          *reinterpret_cast<uint32_t *>(at + p.n_at + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = codes;
+          if (lane % kLanes == 0) at[p.sn_at + (lane / kLanes >> 2) * 512 + row * 16 + (lane / kLanes & 3)] = byte;
+          // the writes above go through the generic proxy, the tensor core reads through the async proxy
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && !(u == 0 && p.withhold_first_load)) mbar_arrive(bar_full(s));
+        }
+        u += kStoreWarps;
+        fetch();
+      }
+      if (++s == p.stages) { s = 0; parity ^= 1; }
+    }
+  }
+  if (warp < kFirstStore) {
   } else if (p.d == 1) {
     constexpr int kUnit = ROWS_M ? 128 / (int)sizeof(T) : 32;   // columns that a warp takes at a time (D[row][oc]: 128 bytes of a row)
     const int me = warp - kFirstStore, quarter = warp & 3, half = me >> 2;
@@ -584,9 +674,10 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
   const int steps = (f->in_channel + kStep - 1) / kStep;
   Geometry best = {false, 16, 1, true};
   double least = 1e300;
-  for (int rows_m = 0; rows_m < 2; ++rows_m) {
+  const bool few = rows <= kFp4DirectRows;  // (the same for quantised rows as for those quantised here: the same sums)
+  for (int rows_m = 0; rows_m < (few ? 1 : 2); ++rows_m) {
     const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
-    for (int nt = 16; nt <= 256; nt *= 2) {
+    for (int nt = 16; nt <= (few ? 16 : 256); nt *= 2) {
       // The scales of a tile begin at its first 32-row group's column, and an MMA takes scales from even columns
       // only (an odd one is a misaligned address): tiles below 64 begin at 0.
       if (nt < 64 && n > nt) continue;
@@ -603,22 +694,23 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
   return best;
 }
 
-template <int FMT, typename T, bool ROWS_M>
+template <int FMT, typename T, bool ROWS_M, bool DIRECT>
 int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
   static bool ready[64] = {};  // per device
   int dev = 0;
   TETRIS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost));
+    TETRIS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<FMT, T, ROWS_M, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost));
     if (dev < 64) ready[dev] = true;
   }
-  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, map_y, p));
+  TETRIS_CUDA_TRY(launch_overlapped(product_kernel<FMT, T, ROWS_M, DIRECT>, dim3(grid), kThreads, smem, st, (unsigned)p.d, map_m, map_n, map_y, p));
   count_launch();
   return TETRIS_OK;
 }
 template <int FMT, typename T>
 int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
-  return rows_m ? launch<FMT, T, true>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false>(map_m, map_n, map_y, p, grid, smem, st);
+  if (p.x) return launch<FMT, T, false, true>(map_m, map_n, map_y, p, grid, smem, st);
+  return rows_m ? launch<FMT, T, true, false>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false, false>(map_m, map_n, map_y, p, grid, smem, st);
 }
 
 // A matrix whose rows are `pitch` bytes apart, in boxes of 128 bytes x `box_rows`.
@@ -635,13 +727,14 @@ int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const voi
 
 }  // namespace
 
-int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const uint8_t *scales, int64_t rows, int exponent, const float *bias,
-                       void *y, int y_type, int64_t ld, int relu, cudaStream_t st) {
+int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
+                       int relu, cudaStream_t st) {
+  const bool direct = !a.codes;
   const Geometry g = choose(f, rows);
   const bool nv = f->format == TETRIS_FP4_NV;
   const int kt = step_tiles(f->format), rt = g.nt > 128 ? 2 : 1, bytes = y_type == TETRIS_FP32 ? 4 : 2;
   ProductParams p = {};
-  p.scales_m = g.rows_m ? scales : f->d_scales; p.scales_n = g.rows_m ? f->d_scales : scales;
+  p.scales_m = g.rows_m ? a.scales : f->d_scales; p.scales_n = g.rows_m ? f->d_scales : a.scales;
   p.bias = bias;
   p.y = y; p.ld = ld;
   p.m_extent = (int)(g.rows_m ? rows : f->out_channel); p.n_extent = (int)(g.rows_m ? f->out_channel : rows);
@@ -674,20 +767,29 @@ int launch_fp4_product(const tetris_fp4_filter *f, const uint8_t *codes, const u
   p.acc1 = p.accs == 2 ? std::min(std::max(g.nt, 32), (p.sf - g.nt) / 32 * 32) : 0;
   const int e = exponent + f->exponent, e0 = std::max(-126, std::min(126, e));
   p.scale = ldexpf(1.f, e0); p.scale1 = ldexpf(1.f, e - e0);
+  p.K = f->in_channel;
+  if (direct) {
+    const int x_bytes = a.x_type == TETRIS_FP32 ? 4 : 2;
+    p.x = a.x; p.x_type = a.x_type; p.x_ld = a.ld;
+    p.x_vec = ((reinterpret_cast<uintptr_t>(a.x) | (uint64_t)(a.ld * x_bytes)) & 15) == 0;
+    p.px.S = 1;
+    if (a.px) p.px = *a.px;
+    fp4_scale_factors(exponent, &p.tensor_scale, &p.sixth, &p.sixth_rest);
+  }
   p.relu = relu;
   // (the distance between rows in a tensor map is below 2^40 bytes)
   p.tma_store = g.rows_m && g.d == 1 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes)) & 15) == 0 && ld * bytes < (1ll << 40);
   p.error_flag = f->d_error;
   p.withhold_first_load = test_injection(&p.spin_limit);
-  CUtensorMap map_w, map_a, map_y = {};
+  CUtensorMap map_w, map_a = {}, map_y = {};
   int rc;
   if ((rc = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, f->d_codes, f->pitch, f->pitch, f->out_channel, g.rows_m ? g.nt : kM)) ||
-      (rc = encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, f->pitch, f->pitch, rows, g.rows_m ? kM : g.nt)) ||
+      (!direct && (rc = encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, f->pitch, f->pitch, rows, g.rows_m ? kM : g.nt))) ||
       (p.tma_store && (rc = encode(&map_y, y_type == TETRIS_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, bytes, y,
                                    f->out_channel, ld * bytes, rows, 32))))
     return rc;
   const CUtensorMap &map_m = g.rows_m ? map_a : map_w, &map_n = g.rows_m ? map_w : map_a;
-  const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, (g.half ? 2 : 1) * f->sm_count));
+  const unsigned grid = (unsigned)(g.d > 1 || direct ? p.total_tiles * g.d : std::min(p.total_tiles, (g.half ? 2 : 1) * f->sm_count));
   const size_t smem = g.half ? kSmemHalf : std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail);
   switch (y_type) {
     case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
