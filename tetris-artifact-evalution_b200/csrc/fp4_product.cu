@@ -668,10 +668,17 @@ struct Geometry {
   bool half;
 };
 
-// The least of an estimate in clocks: waves of tiles, each K step at the longer of its MMAs and its loads
-// (about 44 bytes a clock and SM from L2), the store of the last tile, the meeting of a cluster.
+// The least of an estimate in nanoseconds, whose terms were fitted to 60 shapes (1 to 50000 rows, 64 to 16384
+// columns and channels) in every geometry: over those its choice takes 1.2 % longer than the best, 11 % at worst.
+//   a K step    the longer of its MMAs and its loads (66 bytes a nanosecond and SM)
+//   a tile      the longer of its steps and the store of the one before it; the last store stands alone
+//   a whole SM  a tile of up to 128 columns hands over to the next one 800 ns late; two halves hide that, at 8 %
+//               more per step (1024x4096x4096: 128 columns 13.1 us in halves and 18.1 whole, 256 columns 12.7)
+//   a cluster   its meeting grows with the columns (64x4096x4096: 10.2 us in one slice, 7.6 in four; 16 columns
+//               1x4096x4096: 8.5 and 4.1)
 Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
-  const int steps = (f->in_channel + kStep - 1) / kStep;
+  const int steps = (f->in_channel + kStep - 1) / kStep, sms = f->sm_count;
+  const double row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
   Geometry best = {false, 16, 1, true};
   double least = 1e300;
   const bool few = rows <= kFp4DirectRows;  // (the same for quantised rows as for those quantised here: the same sums)
@@ -682,12 +689,15 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
       // only (an odd one is a misaligned address): tiles below 64 begin at 0.
       if (nt < 64 && n > nt) continue;
       const int64_t tiles = (m + kM - 1) / kM * ((n + nt - 1) / nt);
-      for (int d = 1; d <= 8; d *= 2) {
-        if (d > 1 && (d > steps || nt > 128 || tiles * d > f->sm_count)) continue;
-        const double waves = (double)((tiles * d + f->sm_count - 1) / f->sm_count);
-        const double step = std::max(2.0 * nt, (kM + nt) * 144 / 44.0), store = (rows_m ? 4.0 : 8.0) * nt;
-        const double cost = waves * std::max((double)((steps + d - 1) / d) * step, store) + (d > 1 ? 1500 + 4.0 * nt : store);
-        if (cost < least) { least = cost; best = {rows_m != 0, nt, d, nt <= 64 || (nt == 128 && d == 1)}; }
+      const double step = std::max(2.3 * nt, (kM + nt) * row_bytes / 66.), store = (rows_m ? 5. : 7.) * nt;
+      for (int half = nt <= 128; half >= 0; --half) {
+        for (int d = 1; d <= 8; d *= 2) {
+          if (d > 1 && (d > steps || nt > (half ? 64 : 128) || tiles * d > (half ? 2 : 1) * sms)) break;
+          const double per_sm = (double)((tiles * d + sms - 1) / sms), k = (double)((steps + d - 1) / d) * step;
+          const double cost = per_sm * std::max(half ? 1.08 * k : k, store) + (d > 1 ? 32. * nt : store) +
+                              (half ? 0. : 28. + (nt > 128 ? 0. : 800. * (per_sm - 1)));
+          if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0}; }
+        }
       }
     }
   }
