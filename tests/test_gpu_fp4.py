@@ -214,7 +214,8 @@ PRODUCTS = [  # rows, K, N
     (1, 1, 1), (1, 64, 128), (1, 4096, 300), (2, 31, 3), (3, 100, 129), (5, 15, 130), (8, 256, 128), (9, 257, 64), (15, 33, 31), (16, 512, 256), (17, 128, 96),
     (31, 63, 127), (32, 1024, 255), (33, 255, 1), (48, 2048, 200), (63, 65, 128), (64, 640, 384), (65, 129, 130), (100, 333, 77), (127, 191, 256), (128, 256, 128),
     (129, 511, 129), (160, 96, 640), (192, 1000, 100), (255, 320, 60), (256, 768, 512), (257, 64, 257), (300, 1537, 300), (511, 48, 1000), (640, 16, 16), (1000, 2048, 1000),
-    (2049, 128, 130), (5000, 64, 256), (333, 8192, 260)]
+    (2049, 128, 130), (5000, 64, 256), (333, 8192, 260),
+    (1100, 4096, 2000), (2400, 700, 2300), (4000, 2048, 700)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)

@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "fp4.h"
 #include "fp4_block.h"
@@ -132,28 +133,25 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// Descriptors of shared memory, low word; the high words are constants.
 // K-major codes in 128-byte rows with the 128-byte swizzle, 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t codes_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
+constexpr uint32_t kCodesHigh = 64u | (1u << 14) | (2u << 29);
 // a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart
-__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | (8ull << 32) | (1ull << 46);
-}
+constexpr uint32_t kScalesHigh = 8u | (1u << 14);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | (1u << 16); }
 // 512 bytes of scales into 4 columns of all four lane quarters
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t desc) {
+  asm volatile("{\n.reg .b64 d;\nmov.b64 d, {%1, %2};\ntcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n}" ::"r"(taddr), "r"(desc), "n"(kScalesHigh) : "memory");
 }
 template <int FMT>
-__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  if (FMT == TETRIS_FP4_NV)
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}"
-                 ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
-                 ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint32_t da, uint32_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+#define TETRIS_FP4_MMA(KIND)                                                                                              \
+  asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %7};\nmov.b64 b, {%2, %7};\nsetp.ne.b32 p, %6, 0;\n"  \
+               "tcgen05.mma.cta_group::1.kind::" KIND " [%0], a, b, %3, [%4], [%5], p;\n}"                                 \
+               ::"r"(tmem_d), "r"(da), "r"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kCodesHigh) : "memory")
+  if (FMT == TETRIS_FP4_NV) TETRIS_FP4_MMA("mxf4nvf4.block_scale.scale_vec::4X");
+  else TETRIS_FP4_MMA("mxf4.block_scale.scale_vec::2X");
+#undef TETRIS_FP4_MMA
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -251,7 +249,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(bias_rows) + kBiasBytes);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the warp number as a value that is the same in all lanes for the compiler, too: what the tensor core is told
+  // can then be worked out in uniform registers; 4096x4096x16384 147 -> 144 us)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   auto bar_full = [&](int s) { return smem_u32(&bars[s]); };
   auto bar_empty = [&](int s) { return smem_u32(&bars[kStagesMax + s]); };
   auto bar_pfull = [&](int b) { return smem_u32(&bars[2 * kStagesMax + b]); };
@@ -349,6 +349,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
       __syncwarp();
     };
+    const uint32_t ring0 = desc_low(smem_u32(ring)), stage_step = (uint32_t)p.stage_bytes >> 4;
     int s = 0, slot = 0, free_s = 0, behind = 0;   // behind: steps whose scale slots may still be read
     uint32_t parity = 0, free_parity = 0;
     int i = 0;
@@ -367,11 +368,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         }
         wait(bar_full(s), parity);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes);
-        const uint32_t sfm = tmem + p.sf + slot * p.slot_cols, sfn = sfm + 4 * kTiles;
+        const uint32_t at = ring0 + (uint32_t)s * stage_step;   // (addresses in units of 16 bytes)
+        const uint32_t sfm = tmem + p.sf + slot * p.slot_cols, sfn = sfm + 4 * kTiles, sfn_row = sfn + sf_row;
         const int n = min(kTiles, p.tiles_k - step * kTiles), mmas = step == p.steps - 1 ? p.last_mmas : 4;
+        const uint32_t dsm = at + (p.sm_at >> 4), dsn = at + (p.sn_at >> 4), dn = at + (p.n_at >> 4);
+        const uint32_t more = step > step0;
         if (elect_one()) {
-          const uint64_t dsm = scales_desc(at + p.sm_at), dsn = scales_desc(at + p.sn_at);
 #pragma unroll
           for (int k = 0; k < kTiles; ++k) {
             if (k < n) {
@@ -380,13 +382,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
               if (rt == 2) copy_scales(sfn + 8 * k + 4, dsn + 32 * (kTiles + k));
             }
           }
-          const uint64_t dm = codes_desc(at), dn = codes_desc(at + p.n_at);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j < mmas) {
               const int k = FMT == TETRIS_FP4_NV ? j : j >> 1;
               const uint32_t id = FMT == TETRIS_FP4_NV || !(j & 1) ? idesc : idesc | (2u << 4) | (2u << 29);  // (second half of the scale words)
-              umma_fp4<FMT>(acc, dm + 2 * j, dn + 2 * j, id, sfm + 4 * k, sfn + 4 * rt * k + sf_row, step > step0 || j > 0);
+              umma_fp4<FMT>(acc, at + 2 * j, dn + 2 * j, id, sfm + 4 * k, sfn_row + 4 * rt * k, j == 0 ? more : 1u);
             }
           }
           umma_commit(bar_empty(s));
@@ -669,16 +670,18 @@ struct Geometry {
 };
 
 // The least of an estimate in nanoseconds, whose terms were fitted to 60 shapes (1 to 50000 rows, 64 to 16384
-// columns and channels) in every geometry: over those its choice takes 1.2 % longer than the best, 11 % at worst.
-//   a K step    the longer of its MMAs and its loads (66 bytes a nanosecond and SM)
+// columns and channels) in every geometry: its choice takes 1.5 % longer than the best, 15 % at worst.
+//   a K step    the longer of its MMAs and its loads: 51 bytes a nanosecond for half an SM alone, 2 x 40 for two
+//               halves, 75 for a whole one (16x8192x8192: 12.2 us in 128 halves, 9.5 in 256)
 //   a tile      the longer of its steps and the store of the one before it; the last store stands alone
-//   a whole SM  a tile of up to 128 columns hands over to the next one 800 ns late; two halves hide that, at 8 %
-//               more per step (1024x4096x4096: 128 columns 13.1 us in halves and 18.1 whole, 256 columns 12.7)
-//   a cluster   its meeting grows with the columns (64x4096x4096: 10.2 us in one slice, 7.6 in four; 16 columns
-//               1x4096x4096: 8.5 and 4.1)
+//   a whole SM  hands over to the next tile 500 ns late; two halves hide that
+//               (1024x4096x4096: 128 columns 13.1 us in halves and 18.1 whole, 256 columns 12.7)
+//   a cluster   its meeting grows with the columns (64x4096x4096: 10.2 us in one slice, 7.6 in four)
+//   a launch that leaves no room for the next one's CTAs beside its own takes 600 ns longer
+//               (1x4096x4096: 4.1 us in 128 halves, 5.5 in 256)
 Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
-  const int steps = (f->in_channel + kStep - 1) / kStep, sms = f->sm_count;
-  const double row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
+  const int steps = (f->in_channel + kStep - 1) / kStep;
+  const double sms = f->sm_count, row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
   Geometry best = {false, 16, 1, true};
   double least = 1e300;
   const bool few = rows <= kFp4DirectRows;  // (the same for quantised rows as for those quantised here: the same sums)
@@ -689,13 +692,22 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
       // only (an odd one is a misaligned address): tiles below 64 begin at 0.
       if (nt < 64 && n > nt) continue;
       const int64_t tiles = (m + kM - 1) / kM * ((n + nt - 1) / nt);
-      const double step = std::max(2.3 * nt, (kM + nt) * row_bytes / 66.), store = (rows_m ? 5. : 7.) * nt;
+      const double bytes = (kM + nt) * row_bytes, store = (rows_m ? 5.8 : 9.7) * nt;
       for (int half = nt <= 128; half >= 0; --half) {
         for (int d = 1; d <= 8; d *= 2) {
-          if (d > 1 && (d > steps || nt > (half ? 64 : 128) || tiles * d > (half ? 2 : 1) * sms)) break;
-          const double per_sm = (double)((tiles * d + sms - 1) / sms), k = (double)((steps + d - 1) / d) * step;
-          const double cost = per_sm * std::max(half ? 1.08 * k : k, store) + (d > 1 ? 32. * nt : store) +
-                              (half ? 0. : 28. + (nt > 128 ? 0. : 800. * (per_sm - 1)));
+          if (d > 1 && (d > steps || nt > (half ? 64 : 128) || tiles * d > (half ? 2 : 1) * f->sm_count)) break;
+          const double ctas = (double)tiles * d, k = (double)((steps + d - 1) / d);
+          double cost;
+          if (half && ctas <= sms) {
+            cost = k * std::max(bytes / 51., 1.1 * nt);
+          } else if (half) {
+            const double rounds = ctas <= 4 * sms ? std::max(1., ctas / (2 * sms)) : std::ceil(ctas / (2 * sms) - 0.1);
+            cost = rounds * std::max(k * std::max(bytes / 40., 2.5 * nt), 2.5 * store) + 620.;
+          } else {
+            const double rounds = std::ceil(ctas / sms);
+            cost = rounds * std::max(k * std::max(bytes / 75., 1.1 * nt), store) + (rounds - 1) * (nt > 128 ? 500. : 580.) + 36. + (2 * ctas > sms ? 620. : 0.);
+          }
+          cost += d > 1 ? 100. + 20. * nt : store;
           if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0}; }
         }
       }
