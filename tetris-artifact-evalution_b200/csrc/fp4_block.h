@@ -20,7 +20,7 @@
 namespace tetris {
 
 // codes of 8 values, the first in the lowest 4 bits (RNE, at most 6)
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
+__device__ __forceinline__ uint32_t codes_of(const float *v) {
   uint32_t r;
   asm("{\n.reg .b8 a, b, c, d;\n"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
@@ -41,18 +41,18 @@ __device__ __forceinline__ float e4m3_value(uint8_t b) {
 }
 
 // The values of a thread's part of a block become quotients by the block's scale; returns the scale's byte.
-template <int FMT>
-__device__ __forceinline__ uint8_t scale_block(float (&v)[8], float top, float tensor_scale, float sixth, float sixth_rest) {
+template <int FMT, int N>
+__device__ __forceinline__ uint8_t scale_block(float (&v)[N], float top, float tensor_scale, float sixth, float sixth_rest) {
   if (!(top < __int_as_float(0x7F800000))) {  // codes of 1: the block is NaN whatever it meets
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 1.f;
+    for (int i = 0; i < N; ++i) v[i] = 1.f;
     return FMT == TETRIS_FP4_NV ? 0x7F : 0xFF;
   }
   if (FMT == TETRIS_FP4_MX) {
     const int byte = max((int)(__float_as_uint(top) >> 23) - 2, 0);  // at most 252
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    for (int i = 0; i < N; ++i) v[i] *= inv;
     return (uint8_t)byte;
   }
   const float within = fminf(top, 4096.f * tensor_scale);  // (beyond 2688 the scale stays at its largest)
@@ -61,14 +61,14 @@ __device__ __forceinline__ uint8_t scale_block(float (&v)[8], float top, float t
   if (top > 1e3f * s && s > 0.f) {  // far above what the exponent holds: x / s could leave FP32
     const float most = 1e3f * s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
+    for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
   }
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   if (s == 0.f) r = 0.f;
   const float rest = __fmaf_rn(-r, s, 1.f) * r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __fmaf_rn(v[i], r, v[i] * rest);
+  for (int i = 0; i < N; ++i) v[i] = __fmaf_rn(v[i], r, v[i] * rest);
   return byte;
 }
 

@@ -4,7 +4,7 @@
 //
 // Bound: HBM; what stands in its way is the number of instructions, so a thread keeps one column position
 // and walks down kRows rows, takes 8 values at a time, and finds the largest one of 16-bit types as packed
-// integers.  4096 x 8192: see the figures at the launch.
+// integers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -17,9 +17,9 @@
 namespace tetris {
 namespace {
 
-constexpr int kThreads = 256, kRows = 4;
+constexpr int kThreads = 256, kRows = 2, kRowsBack = 4;  // rows of a thread: quantising, and back
 
-// How a block of threads covers a matrix cut into pieces of 8 columns: 2^lx threads side by side, the others
+// How a block of threads covers a matrix cut into pieces of 8 or 16 columns: 2^lx threads side by side, the others
 // below them, and again `ROWS` times.
 struct Walk {
   int lx;
@@ -48,32 +48,44 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
-// 8 values as they were loaded, and what is asked of them.
+// Neighbouring values as they were loaded (32 bytes), and what is asked of them.
 template <typename T> struct Piece {  // 16-bit types
-  uint4 raw;
-  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const T *src, bool) { raw = *reinterpret_cast<const uint4 *>(src); }
-  __device__ __forceinline__ void set(int k, T v) {
-    const uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t *>(&v) << (16 * (k & 1));
-    (k < 2 ? raw.x : k < 4 ? raw.y : k < 6 ? raw.z : raw.w) |= b;
+  static constexpr int kValues = 16;
+  uint32_t raw[8];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) raw[k] = 0;
   }
+  __device__ __forceinline__ void load(const T *src, bool wide) {
+    if (wide) {
+      asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7]) : "l"(src));
+    } else {
+      *reinterpret_cast<uint4 *>(raw) = reinterpret_cast<const uint4 *>(src)[0];
+      *reinterpret_cast<uint4 *>(raw + 4) = reinterpret_cast<const uint4 *>(src)[1];
+    }
+  }
+  __device__ __forceinline__ void set(int k, T v) { raw[k >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t *>(&v) << (16 * (k & 1)); }
   // Bits of |x|, two values side by side: as integers they are ordered like the numbers, NaN last.
   __device__ __forceinline__ uint32_t top() const {
-    const uint32_t m = 0x7FFF7FFFu;
-    return __vmaxu2(__vmaxu2(raw.x & m, raw.y & m), __vmaxu2(raw.z & m, raw.w & m));
+    uint32_t t = raw[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) t = __vmaxu2(t, raw[k] & 0x7FFF7FFFu);
+    return t;
   }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
   static __device__ __forceinline__ float number(uint32_t t) {
     const uint16_t b = (uint16_t)max(t & 0xFFFFu, t >> 16);
     return to_float(*reinterpret_cast<const T *>(&b));
   }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-    const T *e = reinterpret_cast<const T *>(&raw);
+  __device__ __forceinline__ void values(float (&v)[16]) const {
+    const T *e = reinterpret_cast<const T *>(raw);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = to_float(e[k]);
+    for (int k = 0; k < 16; ++k) v[k] = to_float(e[k]);
   }
 };
 template <> struct Piece<float> {
+  static constexpr int kValues = 8;
   float v[8];
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -105,15 +117,15 @@ template <> struct Piece<float> {
 
 template <typename T, int FMT, bool VEC, bool STRIDED, int ROWS>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams p) {
-  constexpr int kBlock = FMT == TETRIS_FP4_NV ? 16 : 32;
-  constexpr int kLanes = kBlock / 8;                                  // threads of a block of values
+  constexpr int kValues = Piece<T>::kValues;
+  constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / kValues;  // threads of a block of values
   grid_release();
   grid_wait();
   const uint32_t row_block = blockIdx.x / p.walk.col_blocks, col_block = blockIdx.x - row_block * p.walk.col_blocks;
   const uint32_t below = kThreads >> p.walk.lx;
   const uint32_t piece = (col_block << p.walk.lx) + (threadIdx.x & ((1u << p.walk.lx) - 1u));
   const uint32_t row0 = row_block * (below * ROWS) + (threadIdx.x >> p.walk.lx);
-  const int col = (int)piece * 8, left = p.cols - col;                // (may lie behind the last column: zeros)
+  const int col = (int)piece * kValues, left = p.cols - col;          // (may lie behind the last column: zeros)
   const T *x = static_cast<const T *>(p.x) + col;
   Piece<T> in[ROWS];
 #pragma unroll
@@ -128,16 +140,17 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams
       from = ((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S;
     }
     const T *src = x + from * p.ld;
-    if (VEC && left >= 8) {
+    if (VEC && left >= kValues) {
       in[u].load(src, p.wide);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < kValues; ++k)
         if (k < left) in[u].set(k, src[k]);
     }
   }
   const bool has_codes = col / 2 < p.pitch, has_scale = piece % kLanes == 0 && (int)(piece / (4 * kLanes)) < p.tiles;
-  const uint32_t keep = left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u;  // zeros behind the last column
+  auto keep = [](int left) { return left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u; };  // zeros behind the last column
+  const uint32_t keep0 = keep(left), keep1 = keep(left - 8);
   uint8_t *codes = p.codes + col / 2;
   uint8_t *scales = p.scales + (size_t)(piece / (4 * kLanes)) * 512 + piece / kLanes % 4;
 #pragma unroll
@@ -146,12 +159,15 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams
     uint32_t top = in[u].top();
 #pragma unroll
     for (int s = 1; s < kLanes; s *= 2) top = Piece<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, s));
-    float v[8];
+    float v[kValues];
     in[u].values(v);
     const uint8_t byte = scale_block<FMT>(v, Piece<T>::number(top), p.tensor_scale, p.sixth, p.sixth_rest);
-    const uint32_t c = codes_of(v) & keep;
+    const uint32_t c = codes_of(v) & keep0;
     if (row >= p.rows) continue;
-    if (has_codes) *reinterpret_cast<uint32_t *>(codes + row * p.pitch) = c;
+    if (has_codes) {
+      if (kValues == 16) *reinterpret_cast<uint2 *>(codes + row * p.pitch) = make_uint2(c, codes_of(v + kValues - 8) & keep1);
+      else *reinterpret_cast<uint32_t *>(codes + row * p.pitch) = c;
+    }
     if (has_scale) scales[(int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4] = byte;
   }
 }
@@ -263,8 +279,8 @@ int launched(cudaError_t err) {
 }
 
 // Threads side by side for `pieces` of a row: what leaves the fewest of them idle, more rather than fewer.
-// `many`: enough blocks for every SM even with kRows rows a thread (few rows are spread over more threads).
-int plan_walk(uint32_t rows, int64_t pieces, Walk *w, unsigned *blocks, bool *many) {
+// `many`: enough blocks for every SM even with `thread_rows` rows a thread (few rows are spread over more threads).
+int plan_walk(uint32_t rows, int64_t pieces, int thread_rows, Walk *w, unsigned *blocks, bool *many) {
   int64_t least = INT64_MAX;
   for (int lx = 8; lx >= 2; --lx) {
     const int64_t padded = ((pieces + (1 << lx) - 1) >> lx) << lx;
@@ -272,8 +288,8 @@ int plan_walk(uint32_t rows, int64_t pieces, Walk *w, unsigned *blocks, bool *ma
   }
   w->col_blocks = (uint32_t)(least >> w->lx);
   const int64_t below = kThreads >> w->lx;
-  *many = (rows + below * kRows - 1) / (below * kRows) * w->col_blocks >= 2 * 148;
-  const int64_t span = below * (*many ? kRows : 1), n = (rows + span - 1) / span * w->col_blocks;
+  *many = (rows + below * thread_rows - 1) / (below * thread_rows) * w->col_blocks >= 2 * 148;
+  const int64_t span = below * (*many ? thread_rows : 1), n = (rows + span - 1) / span * w->col_blocks;
   if (n > 0x7FFFFFFF) { set_error("a matrix of this size is outside what the kernels cover"); return TETRIS_ERR_UNSUPPORTED; }
   *blocks = (unsigned)n;
   return TETRIS_OK;
@@ -288,14 +304,14 @@ template <typename T, int FMT> int quantize(QuantizeParams p, bool strided, cuda
   p.wide = vector_rows(p.x, p.ld, sizeof(T), 32);
   unsigned blocks;
   bool many;
-  const int rc = plan_walk(p.rows, (int64_t)p.tiles * fp4_block(FMT) / 2, &p.walk, &blocks, &many);
+  const int rc = plan_walk(p.rows, (int64_t)p.tiles * 4 * fp4_block(FMT) / Piece<T>::kValues, kRows, &p.walk, &blocks, &many);
   if (rc) return rc;
   if (strided) return vec ? quantize<T, FMT, true, true>(p, blocks, many, st) : quantize<T, FMT, false, true>(p, blocks, many, st);
   return vec ? quantize<T, FMT, true, false>(p, blocks, many, st) : quantize<T, FMT, false, false>(p, blocks, many, st);
 }
 
 template <typename T, int FMT, bool VEC> int dequantize(const DequantizeParams &p, unsigned blocks, bool many, cudaStream_t st) {
-  return launched(many ? launch_overlapped(dequantize_kernel<T, FMT, VEC, kRows>, dim3(blocks), kThreads, 0, st, 1, p)
+  return launched(many ? launch_overlapped(dequantize_kernel<T, FMT, VEC, kRowsBack>, dim3(blocks), kThreads, 0, st, 1, p)
                        : launch_overlapped(dequantize_kernel<T, FMT, VEC, 1>, dim3(blocks), kThreads, 0, st, 1, p));
 }
 template <typename T, int FMT> int dequantize(DequantizeParams p, cudaStream_t st) {
@@ -303,7 +319,7 @@ template <typename T, int FMT> int dequantize(DequantizeParams p, cudaStream_t s
   p.wide = vector_rows(p.y, p.ld, sizeof(T), 32);
   unsigned blocks;
   bool many;
-  const int rc = plan_walk(p.rows, ((int64_t)p.cols + 7) / 8, &p.walk, &blocks, &many);
+  const int rc = plan_walk(p.rows, ((int64_t)p.cols + 7) / 8, kRowsBack, &p.walk, &blocks, &many);
   if (rc) return rc;
   return vec ? dequantize<T, FMT, true>(p, blocks, many, st) : dequantize<T, FMT, false>(p, blocks, many, st);
 }
