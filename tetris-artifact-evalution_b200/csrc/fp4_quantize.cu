@@ -148,7 +148,9 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams
         if (k < left) in[u].set(k, src[k]);
     }
   }
-  const bool has_codes = col / 2 < p.pitch, has_scale = piece % kLanes == 0 && (int)(piece / (4 * kLanes)) < p.tiles;
+  // pieces cover a row's pitch (whole 32 columns); the last block also writes the zeros that fill its scale tile
+  const bool has_codes = col / 2 < p.pitch, has_scale = has_codes && piece % kLanes == 0;
+  const int fill = has_scale && (col + kLanes * kValues) / 2 >= p.pitch ? 3 - (int)(piece / kLanes % 4) : 0;
   auto keep = [](int left) { return left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u; };  // zeros behind the last column
   const uint32_t keep0 = keep(left), keep1 = keep(left - 8);
   uint8_t *codes = p.codes + col / 2;
@@ -168,7 +170,11 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams
       if (kValues == 16) *reinterpret_cast<uint2 *>(codes + row * p.pitch) = make_uint2(c, codes_of(v + kValues - 8) & keep1);
       else *reinterpret_cast<uint32_t *>(codes + row * p.pitch) = c;
     }
-    if (has_scale) scales[(int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4] = byte;
+    if (has_scale) {
+      uint8_t *s = scales + (int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4;
+      *s = byte;
+      for (int k = 1; k <= fill; ++k) s[k] = 0;
+    }
   }
 }
 
@@ -304,7 +310,7 @@ template <typename T, int FMT> int quantize(QuantizeParams p, bool strided, cuda
   p.wide = vector_rows(p.x, p.ld, sizeof(T), 32);
   unsigned blocks;
   bool many;
-  const int rc = plan_walk(p.rows, (int64_t)p.tiles * 4 * fp4_block(FMT) / Piece<T>::kValues, kRows, &p.walk, &blocks, &many);
+  const int rc = plan_walk(p.rows, p.pitch * 2 / Piece<T>::kValues, kRows, &p.walk, &blocks, &many);
   if (rc) return rc;
   if (strided) return vec ? quantize<T, FMT, true, true>(p, blocks, many, st) : quantize<T, FMT, false, true>(p, blocks, many, st);
   return vec ? quantize<T, FMT, true, false>(p, blocks, many, st) : quantize<T, FMT, false, false>(p, blocks, many, st);
