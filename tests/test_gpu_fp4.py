@@ -465,11 +465,12 @@ def test_filters_from_host_and_device_arrays(tb, torch_cuda, fmt):
 
 def test_refusals_on_the_device(tb, torch_cuda):
     torch = torch_cuda
-    f, _ = filter_and_weights(tb, torch, 64, 128, ref.MX, 1)
-    x = activations(torch, 300, 128, 2)
-    y = torch.full((300, 64), 5.0, device="cuda")
+    f, _ = filter_and_weights(tb, torch, 4096, 4096, ref.MX, 1)
+    x = activations(torch, 300, 4096, 2)
+    y = torch.full((300, 4096), 5.0, device="cuda")
     codes, scales = quantized(tb, torch, x, ref.MX)
     need = tb.fp4_workspace(f, 300)
+    assert need  # (products of fewer values quantise them on their own)
     work = torch.empty(need, dtype=torch.uint8, device="cuda")
     torch.cuda.synchronize()
 
@@ -484,15 +485,15 @@ def test_refusals_on_the_device(tb, torch_cuda):
     refused(lambda: tb.fp4_linear(f, x, y.cpu(), 300, work))
     refused(lambda: tb.fp4_linear(f, x, y, 300, work.cpu()))
     refused(lambda: tb.fp4_linear(f, x, y, 300, work, exponent=2))
-    refused(lambda: tb.fp4_linear(f, x, y, 300, work, bias=torch.zeros(64)))
+    refused(lambda: tb.fp4_linear(f, x, y, 300, work, bias=torch.zeros(4096)))
     refused(lambda: tb.fp4_product(f, codes.cpu(), scales, y, 300))
     refused(lambda: tb.fp4_product(f, codes, scales.cpu(), y, 300))
     refused(lambda: tb.fp4_product(f, codes[1:], scales, y, 300))
     refused(lambda: tb.fp4_product(f, codes, scales, y, -1))
-    refused(lambda: tb.fp4_product(f, codes.data_ptr(), scales, y.data_ptr(), 300, ld=63))
+    refused(lambda: tb.fp4_product(f, codes.data_ptr(), scales, y.data_ptr(), 300, ld=4095))
     refused(lambda: tb.fp4_product(f, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), 300, dtype=9))
-    refused(lambda: tb.fp4_quantize(x.cpu(), codes, scales, 300, 128, ref.MX))
-    refused(lambda: tb.fp4_dequantize(codes, scales, x.cpu(), 300, 128, ref.MX))
+    refused(lambda: tb.fp4_quantize(x.cpu(), codes, scales, 300, 4096, ref.MX))
+    refused(lambda: tb.fp4_dequantize(codes, scales, x.cpu(), 300, 4096, ref.MX))
     refused(lambda: tb.fp4_conv2d(f, x, y, 3, 10, 10, 1, 1, work), 3)
     refused(lambda: tb.fp4_conv2d(f, x, y, 3, 10, 10, 0, 0, work))
     lib = tb.lib()
@@ -501,7 +502,7 @@ def test_refusals_on_the_device(tb, torch_cuda):
     assert lib.tetris_fp4_linear(f.handle, x.data_ptr(), 0, 300, 0, 0, None, None, 0, 0, 0, work.data_ptr(), need, None) == 1
     for call in (lambda: tb.fp4_linear(f, x, y, 301, work), lambda: tb.fp4_linear(f, x[:, :100], y, 300, work),
                  lambda: tb.fp4_linear(f, x.double(), y, 300, work), lambda: tb.fp4_product(f, codes, scales, y[:299], 300),
-                 lambda: tb.fp4_linear(f, x, y, 300, work, bias=torch.zeros(63, device="cuda")),
+                 lambda: tb.fp4_linear(f, x, y, 300, work, bias=torch.zeros(4095, device="cuda")),
                  lambda: tb.fp4_conv2d(f, x, y, 4, 10, 10, 1, 0, work), lambda: tb.fp4_conv2d(f, x.half(), y, 3, 10, 10, 1, 0, work)):
         with pytest.raises(ValueError):
             call()

@@ -59,12 +59,14 @@ int launch_fp4_largest(const void *x, int x_type, int64_t n, unsigned *d_bits, c
 // fp4_product.cu
 struct Fp4Rows {             // activations of a product
   const uint8_t *codes, *scales;  // quantised ...
-  const void *x;             // ... or, where codes is null, as they are: at most kFp4DirectRows rows
+  const void *x;             // ... or, where codes is null, as they are
   int x_type;
   int64_t ld;
   const Fp4Pixels *px;
 };
-constexpr int kFp4DirectRows = 4;  // up to here a product quantises its activations itself
+// whether a product of so many rows quantises them itself (else they are quantised into a workspace first); its sums
+// are the same either way
+bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows);
 int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
                        int relu, cudaStream_t st);
 

@@ -62,7 +62,7 @@ int check_filter(const tetris_fp4_filter *f) {
 
 int64_t workspace_codes(const tetris_fp4_filter *f, int64_t rows) { return (rows * f->pitch + 255) / 256 * 256; }
 int64_t workspace_bytes(const tetris_fp4_filter *f, int64_t rows) {
-  return rows <= kFp4DirectRows ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
+  return rows == 0 || fp4_product_direct(f, rows) ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
 }
 
 // Checks that all products share; the filter's device is current.

@@ -13,8 +13,8 @@
 //     zeros past both ends) and bulk copies of the scales, into one ring;
 //   * warp 1 (one elected lane): scales from shared into tensor memory (tcgen05.cp), then 4 MMAs;
 //   * eight storing warps: accumulator -> scale, bias, ReLU -> output, beside the next tile's MMAs.
-// Up to 4 rows that are not quantised yet: the storing warps first turn them into codes and scales in shared
-// memory, a row's 256 values of a K step per warp, while the filter is on its way.
+// Rows that are not quantised yet (DIRECT): before the storing warps store a tile they turn its rows into codes and
+// scales in shared memory, K step by K step, while the filter is on its way.
 // Tensor memory: two accumulators.  With N = 256 two of them and the scales exceed 512 columns, so the
 // second one lies over the end of the first; the storing warps empty the shared columns first and the next
 // tile starts once those are free.
@@ -71,6 +71,8 @@ struct ProductParams {
   int x_type, x_vec, K;
   int64_t x_ld;
   Fp4Pixels px;            // (S > 1: a row is a pixel of a strided layer)
+  Fp4Div by_OH, by_OW;
+  int lx, unit_log;        // log2 of the lanes of a row, of the units (32 lanes) of a tile's rows in a K step
   float tensor_scale, sixth, sixth_rest;  // as in the quantisation
   int relu;
   int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows)
@@ -234,7 +236,7 @@ __device__ __forceinline__ void load8(const ProductParams &p, int64_t at, int le
   for (int k = 0; k < 8; ++k) v[k] = p.x_type == TETRIS_BF16 ? __uint_as_float((uint32_t)h[k] << 16) : __half2float(__ushort_as_half(h[k]));
 }
 
-// DIRECT: the rows (on the N side, at most kFp4DirectRows) are quantised here.
+// DIRECT: the rows are quantised here (with the filter on the M side at most 64 at a time, else 128).
 template <int FMT, typename T, bool ROWS_M, bool DIRECT>
 __global__ void __launch_bounds__(kThreads, 2)
 product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_n, const __grid_constant__ CUtensorMap map_y,
@@ -285,7 +287,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   };
   auto load_filter = [&](int s, int step) {
     const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-    mbar_expect_tx(bar, DIRECT ? (uint32_t)(kM * 128 + scale_tiles(step) * 512)
+    mbar_expect_tx(bar, DIRECT ? (uint32_t)((ROWS_M ? p.nt : kM) * 128 + scale_tiles(step) * 512)
                                : (uint32_t)((kM + p.nt) * 128 + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
     if (ROWS_M) load_n(at, bar, step); else load_m(at, bar, step);
   };
@@ -297,7 +299,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   };
 
   if (tid == 0) {
-    for (int s = 0; s < kStagesMax; ++s) { mbar_init(bar_full(s), DIRECT ? 1 + p.n_extent : 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < kStagesMax; ++s) { mbar_init(bar_full(s), DIRECT ? 1 + kStoreWarps : 1); mbar_init(bar_empty(s), 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(bar_pfull(b), 1); mbar_init(bar_pempty(b), kStoreWarps); mbar_init(bar_shared(b), kStoreWarps); }
     mbar_init(bar_drain(), 1);
     mbar_init(bar_sums(), 1);
@@ -357,7 +359,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       decode(p, t, m0, n0);
       const int b = i & acc_log;
       const uint32_t acc = tmem + (b ? p.acc1 : 0);
-      const uint32_t sf_row = (uint32_t)(n0 & 127) >> 5;   // the tile's first 32-row group within its scale tile: 0 or 2
+      const uint32_t sf_row = DIRECT && !ROWS_M ? 0u : (uint32_t)(n0 & 127) >> 5;   // the tile's first 32-row group within its scale tile: 0 or 2
       if (i > acc_log) wait(bar_pempty(b), ((i >> acc_log) & 1) ^ 1);
       if (over && i >= 1) wait(bar_shared(b ^ 1), ((i - 1) >> 1) & 1);
       for (int step = step0; step < step1; ++step) {
@@ -400,54 +402,69 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       }
     }
   }
-  if (DIRECT && warp >= kFirstStore) {
-    // Unit u: row u & (2^rows_log - 1) of K step u >> rows_log; warp w takes units w, w + 8, ..., a lane 8 values.
-    // Every warp walks all steps and waits for each stage that is used again: a wait for a barrier's phase by its parity
-    // only means something to who has seen the phase before.
-    constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8;
-    const int rows_log = p.n_extent > 2 ? 2 : p.n_extent - 1, units = (step1 - step0) << rows_log;
-    int u = warp - kFirstStore, s = 0;
-    uint32_t parity = 1;
-    float v[8];
-    auto fetch = [&]() {  // the values of unit u
-      const int step = step0 + (u >> rows_log), row = u & ((1 << rows_log) - 1), col = step * kStep + lane * 8;
-      int64_t from = row;
-      if (p.px.S > 1) {
-        const int y = row / p.px.OW, n = y / p.px.OH;
-        from = ((int64_t)n * p.px.H + (int64_t)(y - n * p.px.OH) * p.px.S) * p.px.W + (int64_t)(row - y * p.px.OW) * p.px.S;
-      }
-      load8(p, from * p.x_ld + col, u < units && row < p.n_extent ? p.K - col : 0, v);
+  // DIRECT: the storing warps quantise the rows r0, ... of a tile.  Unit u: 32 >> (5 - lx) lanes' rows of K step
+  // u >> unit_log; warp w takes units w, w + 8, ..., four at a time so that their loads overlap, a lane 8 values.  Every
+  // warp enters every step, waits for its stage and arrives once it is done with it: a wait for a barrier's phase by its
+  // parity only means something to who has seen the phase before.
+  int c_stage = 0;
+  uint32_t c_parity = 1;
+  bool c_withhold = p.withhold_first_load && warp == kFirstStore;
+  auto convert = [&](int r0) {
+    constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8, kAtOnce = 4;
+    const int extent = ROWS_M ? p.m_extent : p.n_extent, units = (step1 - step0) << p.unit_log;
+    const int lane_col = lane & ((1 << p.lx) - 1), lane_row = lane >> p.lx, unit_rows = 5 - p.lx;
+    int step = 0;
+    mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
+    auto leave = [&]() {  // this warp is done with the step
+      // (the writes went through the generic proxy, the tensor core reads through the async proxy)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !c_withhold) mbar_arrive(bar_full(c_stage));
+      c_withhold = false;
+      if (++c_stage == p.stages) { c_stage = 0; c_parity ^= 1; }
     };
-    fetch();
 #pragma unroll 1
-    for (int step = step0; step < step1; ++step) {
-      if (step - step0 >= p.stages) mbar_wait(bar_empty(s), parity, abort_flag);
-      if (u >> rows_log == step - step0) {
-        const int row = u & ((1 << rows_log) - 1);
-        if (row < p.n_extent) {
-          uint32_t top = 0;
+    for (int u0 = warp - kFirstStore; u0 < units; u0 += kStoreWarps * kAtOnce) {
+      float v[kAtOnce][8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);  // (as integers: NaN last)
-          __syncwarp();
-#pragma unroll
-          for (int l = 1; l < kLanes; l *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, l));
-          const uint8_t byte = scale_block<FMT>(v, __uint_as_float(top), p.tensor_scale, p.sixth, p.sixth_rest);
-          const int left = p.K - step * kStep - lane * 8;
-          const uint32_t codes = codes_of(v) & (left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u);
-          unsigned char *at = ring + (size_t)s * p.stage_bytes;
-          *reinterpret_cast<uint32_t *>(at + p.n_at + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = codes;
-          if (lane % kLanes == 0) at[p.sn_at + (lane / kLanes >> 2) * 512 + row * 16 + (lane / kLanes & 3)] = byte;
-          // the writes above go through the generic proxy, the tensor core reads through the async proxy
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && !(u == 0 && p.withhold_first_load)) mbar_arrive(bar_full(s));
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int u = u0 + q * kStoreWarps, row = r0 + ((u & ((1 << p.unit_log) - 1)) << unit_rows) + lane_row;
+        const int col = (step0 + (u >> p.unit_log)) * kStep + lane_col * 8;
+        int64_t from = row;
+        if (p.px.S > 1) {
+          const uint32_t y = fp4_quot((uint32_t)row, p.by_OW), ox = (uint32_t)row - y * p.px.OW, n = fp4_quot(y, p.by_OH), oy = y - n * p.px.OH;
+          from = ((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S;
         }
-        u += kStoreWarps;
-        fetch();
+        load8(p, from * p.x_ld + col, u < units && row < extent ? p.K - col : 0, v[q]);
       }
-      if (++s == p.stages) { s = 0; parity ^= 1; }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int u = u0 + q * kStoreWarps;
+        if (u >= units) break;
+        for (; step < u >> p.unit_log; ++step) {
+          leave();
+          mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
+        }
+        __syncwarp();
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[q][k]) & 0x7FFFFFFFu);  // (as integers: NaN last)
+#pragma unroll
+        for (int l = 1; l < kLanes; l *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, l));
+        const uint8_t byte = scale_block<FMT>(v[q], __uint_as_float(top), p.tensor_scale, p.sixth, p.sixth_rest);
+        const int row = ((u & ((1 << p.unit_log) - 1)) << unit_rows) + lane_row, left = p.K - (step0 + step) * kStep - lane_col * 8, blk = lane_col / kLanes;
+        const uint32_t codes = codes_of(v[q]) & (left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u);
+        unsigned char *at = ring + (size_t)c_stage * p.stage_bytes;
+        *reinterpret_cast<uint32_t *>(at + (ROWS_M ? 0 : p.n_at) + row * 128 + (((lane_col >> 2) ^ (row & 7)) << 4) + (lane_col & 3) * 4) = codes;
+        if (lane_col % kLanes == 0) at[(ROWS_M ? p.sm_at : p.sn_at) + (blk >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (blk & 3)] = byte;
+      }
     }
-  }
+    for (; step < step1 - step0 - 1; ++step) {
+      leave();
+      mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
+    }
+    leave();
+  };
   if (warp < kFirstStore) {
   } else if (p.d == 1) {
     constexpr int kUnit = ROWS_M ? 128 / (int)sizeof(T) : 32;   // columns that a warp takes at a time (D[row][oc]: 128 bytes of a row)
@@ -461,6 +478,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     for (int t = tile0; t < p.total_tiles; t += tile_step, ++i) {
       const int b = i & acc_log, mq = m0 + quarter * 32, m = mq + lane, n_first = n0;
       const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
+      if (DIRECT) convert(ROWS_M ? m0 : n0);
       if (!mbar_try_wait(bar_pfull(b), (i >> acc_log) & 1)) mbar_wait(bar_pfull(b), (i >> acc_log) & 1, abort_flag);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -567,6 +585,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     const int quarter = warp & 3, half = (warp - kFirstStore) >> 2, per = 1 << p.per_log;
     decode(p, tile0, m0, n0);
     const int live = min(p.nt, p.n_extent - n0);
+    if (DIRECT) convert(ROWS_M ? m0 : n0);
     bool ok = __all_sync(0xffffffffu, mbar_wait(bar_pfull(0), 0, abort_flag));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     float *out = reinterpret_cast<float *>(ring);
@@ -663,6 +682,22 @@ EncodeFn get_encode() {
 constexpr size_t kSmemMost = 227 * 1024, kSmemHalf = 113 * 1024;   // (1 KB of either goes into the ring's alignment)
 constexpr size_t kSmemLeast = 117 * 1024;
 
+// A product quantises its rows itself where a storing warp has at most this many units of it to do.  A unit takes such a
+// warp about 0.5 us, which the filter's loads hide in part; a launch of its own takes 2 us of the device, in part hidden,
+// too, and 2.2 us of the host (16x1024x1024, 2 units: 4.8 us on the device and 6.3 on the host in one launch, 4.4 and
+// 8.6 in two; 16x8192x8192, 16 units: 19 and 10 us on the device).
+constexpr int kDirectUnits = 4;
+
+// How the rows of a tile are cut into units of a warp: 2^lx lanes take a row's part of a K step.
+struct Units {
+  int lx, log;             // log: units of a K step
+};
+Units units_of(int cols, int64_t tile_rows) {
+  Units u = {cols <= 64 ? 3 : cols <= 128 ? 4 : 5, 0};
+  while ((int64_t)(32 >> u.lx) << u.log < tile_rows) ++u.log;
+  return u;
+}
+
 struct Geometry {
   bool rows_m;
   int nt, d;
@@ -684,10 +719,9 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
   const double sms = f->sm_count, row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
   Geometry best = {false, 16, 1, true};
   double least = 1e300;
-  const bool few = rows <= kFp4DirectRows;  // (the same for quantised rows as for those quantised here: the same sums)
-  for (int rows_m = 0; rows_m < (few ? 1 : 2); ++rows_m) {
+  for (int rows_m = 0; rows_m < 2; ++rows_m) {
     const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
-    for (int nt = 16; nt <= (few ? 16 : 256); nt *= 2) {
+    for (int nt = 16; nt <= 256; nt *= 2) {
       // The scales of a tile begin at its first 32-row group's column, and an MMA takes scales from even columns
       // only (an odd one is a misaligned address): tiles below 64 begin at 0.
       if (nt < 64 && n > nt) continue;
@@ -731,7 +765,8 @@ int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap
 }
 template <int FMT, typename T>
 int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
-  if (p.x) return launch<FMT, T, false, true>(map_m, map_n, map_y, p, grid, smem, st);
+  if (p.x)
+    return rows_m ? launch<FMT, T, true, true>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false, true>(map_m, map_n, map_y, p, grid, smem, st);
   return rows_m ? launch<FMT, T, true, false>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false, false>(map_m, map_n, map_y, p, grid, smem, st);
 }
 
@@ -748,6 +783,15 @@ int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const voi
 }
 
 }  // namespace
+
+bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows) {
+  const Geometry g = choose(f, rows);
+  const int64_t tiles = ((g.rows_m ? rows : f->out_channel) + kM - 1) / kM * (((g.rows_m ? f->out_channel : rows) + g.nt - 1) / g.nt);
+  if (g.nt > (g.rows_m ? 128 : 64) || tiles * g.d > (g.half ? 2 : 1) * f->sm_count) return false;  // (one tile per CTA)
+  const Units u = units_of(f->in_channel, std::min<int64_t>(rows, g.rows_m ? kM : g.nt));
+  const int steps = ((f->in_channel + kStep - 1) / kStep + g.d - 1) / g.d;
+  return ((int64_t)steps << u.log) <= kDirectUnits * kStoreWarps;
+}
 
 int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
                        int relu, cudaStream_t st) {
@@ -795,7 +839,12 @@ int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t row
     p.x = a.x; p.x_type = a.x_type; p.x_ld = a.ld;
     p.x_vec = ((reinterpret_cast<uintptr_t>(a.x) | (uint64_t)(a.ld * x_bytes)) & 15) == 0;
     p.px.S = 1;
-    if (a.px) p.px = *a.px;
+    if (a.px) {
+      p.px = *a.px;
+      p.by_OH = fp4_div((uint32_t)a.px->OH); p.by_OW = fp4_div((uint32_t)a.px->OW);
+    }
+    const Units u = units_of(p.K, std::min<int64_t>(rows, g.rows_m ? kM : g.nt));
+    p.lx = u.lx; p.unit_log = u.log;
     fp4_scale_factors(exponent, &p.tensor_scale, &p.sixth, &p.sixth_rest);
   }
   p.relu = relu;
@@ -811,7 +860,7 @@ int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t row
                                    f->out_channel, ld * bytes, rows, 32))))
     return rc;
   const CUtensorMap &map_m = g.rows_m ? map_a : map_w, &map_n = g.rows_m ? map_w : map_a;
-  const unsigned grid = (unsigned)(g.d > 1 || direct ? p.total_tiles * g.d : std::min(p.total_tiles, (g.half ? 2 : 1) * f->sm_count));
+  const unsigned grid = (unsigned)(g.d > 1 ? p.total_tiles * g.d : std::min(p.total_tiles, (g.half ? 2 : 1) * f->sm_count));
   const size_t smem = g.half ? kSmemHalf : std::max(kSmemLeast, (size_t)p.stages * p.stage_bytes + tail);
   switch (y_type) {
     case TETRIS_FP32: return nv ? launch<TETRIS_FP4_NV, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st) : launch<TETRIS_FP4_MX, float>(g.rows_m, map_m, map_n, map_y, p, grid, smem, st);
