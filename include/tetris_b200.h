@@ -398,8 +398,9 @@ int tetris_fp4_filter_check(const tetris_fp4_filter_t *f);
  *                       tetris_fp4_quantize and tetris_fp4_product)
  *   tetris_fp4_conv2d   the 1x1 layer: FP32 NHWC in and out as tetris_conv2d_launch, padding must be 0
  * `d_workspace` holds the quantised activations: tetris_fp4_workspace(f, rows) bytes (rows = N * OH * OW
- * for the layer), 16-byte aligned, NULL where that is 0; free again when the call has passed on
- * its stream.
+ * for the layer), 16-byte aligned.  0 bytes (NULL) where so few rows are quantised by the product itself, in one
+ * launch.  It is free again when the call has passed on its stream; calls that can run at the same time (other
+ * streams, graphs that are replayed side by side) each need their own.
  */
 int tetris_fp4_product(const tetris_fp4_filter_t *f, const void *d_codes, const void *d_scales, int64_t rows, int exponent,
                        const float *d_bias, void *d_y, int y_type, int64_t ld, int flags, void *stream);
@@ -412,8 +413,8 @@ int tetris_fp4_conv2d(const tetris_fp4_filter_t *f, const float *d_input_nhwc, f
                       void *d_workspace, int64_t workspace_bytes, void *stream);
 
 /*
- * Number of convolution kernels the library has launched in this process so far (every variant,
- * every device and thread; tuning launches included).  No counterpart in the reference; lets a
+ * Number of convolution kernels and 4-bit products the library has launched in this process so far (every
+ * variant, every device and thread; tuning launches included).  No counterpart in the reference; lets a
  * harness check that a timing loop really issued warm + repeat launches.
  */
 unsigned long long tetris_launch_count(void);

@@ -539,3 +539,63 @@ def test_bounded_wait_gives_up_and_the_next_product_passes(tb, torch_cuda, rows)
     f.check()
     want, terms = reference_product(x, w, ref.NV, 0, f.exponent_)
     check_product(y, want, terms, k, torch)
+
+
+def test_offsets_past_32_bits(tb, torch_cuda):
+    """17 GB of activations, 4.3 GB of codes: the last rows come out as they do on their own."""
+    torch = torch_cuda
+    cols, rows, n, part = 16384, 530000, 48, 1000
+    base = activations(torch, part, cols, 5, spread=1.0, dtype="bf16")
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x.view(rows // part, part, cols)[:] = base
+    f, w = filter_and_weights(tb, torch, n, cols, ref.MX, 6)
+    want_codes, want_scales = quantized(tb, torch, base, ref.MX)
+    codes, scales = [torch.empty(s, dtype=torch.uint8, device="cuda") for s in tb.fp4_sizes(rows, cols, ref.MX)]
+    tb.fp4_quantize(x, codes, scales, rows, cols, ref.MX)
+    pitch = ref.pitch(cols)
+    assert torch.equal(codes[-part * pitch:], want_codes[:part * pitch])
+    y = torch.empty(rows, n, device="cuda")
+    tb.fp4_product(f, codes, scales, y, rows)
+    f.check()
+    check_product(y[-part:], *reference_product(base, w, ref.MX, 0, 0), cols, torch)
+    assert torch.equal(y[-part:], y[:part])
+    x.zero_()
+    tb.fp4_dequantize(codes, scales, x, rows, cols, ref.MX)
+    back = torch.empty_like(base)
+    tb.fp4_dequantize(want_codes, want_scales, back, part, cols, ref.MX)
+    assert torch.equal(x[-part:], back)
+
+
+def test_first_call_inside_a_capture(torch_cuda):
+    """A process whose first product is captured: nothing on the launch path needs an earlier call."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path.insert(0, %r)
+from conftest import load_package
+import torch
+tb = load_package()
+w = torch.randn(300, 512, device='cuda')
+f = tb.Fp4Filter(w, 512, 300)
+x, y = torch.randn(700, 512, device='cuda'), torch.zeros(700, 300, device='cuda')
+z = torch.zeros(2, 300, device='cuda')
+room = torch.empty(tb.fp4_workspace(f, 700), dtype=torch.uint8, device='cuda')
+torch.cuda.synchronize()
+s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    tb.fp4_linear(f, x, y, 700, room, cuda_stream=s)
+    tb.fp4_linear(f, x[:2], z, 2, cuda_stream=s)
+g.replay()
+torch.cuda.synchronize()
+f.check()
+a = torch.empty_like(y)
+tb.fp4_linear(f, x, a, 700, room)
+assert torch.equal(a, y) and bool(y.abs().sum() > 0)
+tb.fp4_linear(f, x[:2], a, 2)
+assert torch.equal(a[:2], z)
+print('captured')
+""" % os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]

@@ -279,6 +279,7 @@ int tetris_fp4_product(const tetris_fp4_filter_t *f, const void *d_codes, const 
   int rc = check_filter(f);
   if (rc) return rc;
   DeviceGuard guard(f->device);
+  if (!guard.ok) { set_error("cudaSetDevice(%d) failed", f->device); return TETRIS_ERR_CUDA; }
   if ((rc = check_product(f, rows, exponent, d_bias, d_y, y_type, &ld, flags)) || rows == 0) return rc;
   if ((rc = check_memory("codes", d_codes, f->device, 16)) || (rc = check_memory("scales", d_scales, f->device, 16))) return rc;
   return launch_fp4_product(f, {static_cast<const uint8_t *>(d_codes), static_cast<const uint8_t *>(d_scales), nullptr, 0, 0, nullptr}, rows, exponent,
@@ -298,6 +299,7 @@ int tetris_fp4_linear(const tetris_fp4_filter_t *f, const void *d_x, int x_type,
   int rc = check_filter(f);
   if (rc) return rc;
   DeviceGuard guard(f->device);
+  if (!guard.ok) { set_error("cudaSetDevice(%d) failed", f->device); return TETRIS_ERR_CUDA; }
   return linear(f, d_x, x_type, rows, ld_x, nullptr, exponent, d_bias, d_y, y_type, ld_y, flags, d_workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
@@ -312,6 +314,7 @@ int tetris_fp4_conv2d(const tetris_fp4_filter_t *f, const float *d_input_nhwc, f
   }
   if (padding != 0) { set_error("a 4-bit layer has no padding, got %d", padding); return TETRIS_ERR_UNSUPPORTED; }
   DeviceGuard guard(f->device);
+  if (!guard.ok) { set_error("cudaSetDevice(%d) failed", f->device); return TETRIS_ERR_CUDA; }
   const Fp4Pixels px = {img_h, img_w, (img_h - 1) / stride + 1, (img_w - 1) / stride + 1, stride};
   const int64_t image = (int64_t)px.OH * px.OW;
   if (batch_size && image > kMaxRows / batch_size) { set_error("%d images of %dx%d are more rows than the kernels cover", batch_size, px.OH, px.OW); return TETRIS_ERR_UNSUPPORTED; }

@@ -3,11 +3,16 @@
 // tcgen05.mma with block scales: kind::mxf4 (32 values a scale, E8M0) and kind::mxf4nvf4 (16 a scale,
 // E4M3), both 64 values of K per instruction, FP32 accumulators in tensor memory.
 //
+// What bounds it: large products the tensor cores and the card's power (4096x4096x16384, MX: 3.8 to 4.2 PFLOP/s at
+// 1.6 to 1.9 GHz and 1000 W; the MMAs alone, without loads and copies of scales, 5.5); few rows the reading of the
+// filter (16x8192x8192, NV: 9.4 us, 4.1 TB/s); layers with few columns the writing of the output (50176x64x256: 12.1 us,
+// 4.4 TB/s); small products the launch (1x2048x1000: 3 us).
+//
 // Which operand is on the M side (128 lanes of tensor memory) depends on the number of rows.
 //   Few rows: the filter, D[oc][row].  16 to 64 rows cost a narrow N instead of an empty M; a lane is a channel,
 //   and 32 lanes store 32 neighbouring values of an output row.
-//   Many rows: the rows, D[row][oc].  A lane then holds neighbouring values of its row and stores 32 bytes at a
-//   time.
+//   Many rows: the rows, D[row][oc].  A lane then holds neighbouring values of its row; a warp stages 32 rows x 128
+//   bytes, which leave as whole lines through a TMA store (each lane storing its own 32 bytes: 3.5 TB/s against 4.9).
 // Roles:
 //   * warp 0 (one thread): per K step of 256 TMA loads of the tile's codes (128 bytes a row, 128-byte swizzle,
 //     zeros past both ends) and bulk copies of the scales, into one ring;
@@ -15,19 +20,23 @@
 //   * eight storing warps: accumulator -> scale, bias, ReLU -> output, beside the next tile's MMAs.
 // Rows that are not quantised yet (DIRECT): before the storing warps store a tile they turn its rows into codes and
 // scales in shared memory, K step by K step, while the filter is on its way.
-// Tensor memory: two accumulators.  With N = 256 two of them and the scales exceed 512 columns, so the
-// second one lies over the end of the first; the storing warps empty the shared columns first and the next
-// tile starts once those are free.
+// Tensor memory: two accumulators (one for 128 columns in half an SM).  With N = 256 two of them and the scales
+// exceed 512 columns, so the second one lies over the end of the first; the storing warps empty the shared columns
+// first and the next tile starts once those are free.
 // Scales lie in slots of tensor memory that are written again only when the MMAs that read them are done.
-// Few tiles: the K range is cut over a cluster of up to 8 CTAs, whose sums are pushed into the shared memory
-// of the CTA that owns a column (asynchronous stores that count on its barrier) and added in slice order:
-// bit-reproducible, no workspace.
+// Few tiles: the K range is cut over a cluster of up to 8 CTAs, whose sums are copied into the shared memory of the
+// CTA that owns a column (one bulk copy per owner, counted on its barrier) and added in slice order: bit-reproducible,
+// no workspace.
 // Every barrier wait is bounded; on a timeout an error flag is raised, all roles drain, tensor memory is
 // freed and the kernel returns; tetris_fp4_filter_check reports it.
+// Tried and dropped: pairs of CTAs on a tile of 256 x 256 (cta_group::2, each stage's arrival passed on to the CTA that
+// issues: 173 us for 4096x4096x16384 against 138), scales copied a step ahead of the MMAs (181), warps of their own that
+// quantise rows of large layers (50176x64x256 15.5 us against 19.4 in two launches, 12544x256x512 20.1 against 12.5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "fp4.h"
@@ -752,7 +761,7 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
 
 template <int FMT, typename T, bool ROWS_M, bool DIRECT>
 int launch(const CUtensorMap &map_m, const CUtensorMap &map_n, const CUtensorMap &map_y, const ProductParams &p, unsigned grid, size_t smem, cudaStream_t st) {
-  static bool ready[64] = {};  // per device
+  static std::atomic<bool> ready[64];  // per device
   int dev = 0;
   TETRIS_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
