@@ -446,6 +446,8 @@ def _fp4_type(x, dtype, what):
     if type(x) is int:
         return FP32 if dtype is None else dtype
     t = _fp4_type_of.get(x.dtype)
+    if t is not None and dtype is None:
+        return t
     if t is None:
         t = _FP4_TYPES.get(str(x.dtype))
         if t is None:
@@ -596,9 +598,12 @@ def fp4_product(fp4_filter, codes, scales, output, rows, exponent=0, bias=None, 
     f = fp4_filter
     need = _fp4_storage(rows, f.in_channel_, f.format_)
     y, ld = _fp4_dense(output, rows, f.out_channel_, ld, "the output")
-    _check(lib().tetris_fp4_product(f.handle, _fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"), rows,
-                                    exponent, _fp4_bias(bias, f.out_channel_), y, _fp4_type(output, dtype, "the output"), ld,
-                                    FUSE_RELU if relu else 0, _stream_ptr(cuda_stream)))
+    status = (_lib or lib()).tetris_fp4_product(
+        f._handle or f.handle, _fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"), rows, exponent,
+        None if bias is None else _fp4_bias(bias, f.out_channel_), y, _fp4_type(output, dtype, "the output"), ld,
+        FUSE_RELU if relu else 0, None if cuda_stream is None else _stream_ptr(cuda_stream))
+    if status:
+        _check(status)
 
 
 def fp4_workspace(fp4_filter, rows):
@@ -628,10 +633,10 @@ def fp4_linear(fp4_filter, input, output, rows, workspace=None, exponent=0, bias
     x, ld_input = _fp4_dense(input, rows, f.in_channel_, ld_input, "the input")
     y, ld_output = _fp4_dense(output, rows, n, ld_output, "the output")
     room, size = _fp4_room(workspace)
-    status = lib().tetris_fp4_linear(f.handle, x, _fp4_type(input, input_dtype, "the input"), rows, ld_input, exponent,
-                                     None if bias is None else _fp4_bias(bias, n), y,
-                                     _fp4_type(output, output_dtype, "the output"), ld_output, FUSE_RELU if relu else 0, room, size,
-                                     None if cuda_stream is None else _stream_ptr(cuda_stream))
+    status = (_lib or lib()).tetris_fp4_linear(
+        f._handle or f.handle, x, _fp4_type(input, input_dtype, "the input"), rows, ld_input, exponent,
+        None if bias is None else _fp4_bias(bias, n), y, _fp4_type(output, output_dtype, "the output"), ld_output,
+        FUSE_RELU if relu else 0, room, size, None if cuda_stream is None else _stream_ptr(cuda_stream))
     if status:
         _check(status)
 

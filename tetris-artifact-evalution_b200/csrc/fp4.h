@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "internal.h"
 
 struct tetris_fp4_filter {
@@ -13,6 +15,8 @@ struct tetris_fp4_filter {
   int64_t pitch, code_bytes, scale_bytes;
   uint8_t *d_codes, *d_scales;
   int *d_error;            // raised by a product that gave up on a barrier wait
+  // geometries of the last numbers of rows (fp4_product.cu): the number in the upper 40 bits, 0: none yet
+  mutable std::atomic<uint64_t> plans[8];
 };
 
 namespace tetris {

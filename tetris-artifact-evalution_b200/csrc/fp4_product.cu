@@ -711,6 +711,7 @@ struct Geometry {
   bool rows_m;
   int nt, d;
   bool half;
+  bool direct;             // rows that come as they are: quantised by the product
 };
 
 // The least of an estimate in nanoseconds, whose terms were fitted to 60 shapes (1 to 50000 rows, 64 to 16384
@@ -723,10 +724,10 @@ struct Geometry {
 //   a cluster   its meeting grows with the columns (64x4096x4096: 10.2 us in one slice, 7.6 in four)
 //   a launch that leaves no room for the next one's CTAs beside its own takes 600 ns longer
 //               (1x4096x4096: 4.1 us in 128 halves, 5.5 in 256)
-Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
+Geometry estimate(const tetris_fp4_filter *f, int64_t rows) {
   const int steps = (f->in_channel + kStep - 1) / kStep;
   const double sms = f->sm_count, row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
-  Geometry best = {false, 16, 1, true};
+  Geometry best = {false, 16, 1, true, false};
   double least = 1e300;
   for (int rows_m = 0; rows_m < 2; ++rows_m) {
     const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
@@ -751,12 +752,33 @@ Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
             cost = rounds * std::max(k * std::max(bytes / 75., 1.1 * nt), store) + (rounds - 1) * (nt > 128 ? 500. : 580.) + 36. + (2 * ctas > sms ? 620. : 0.);
           }
           cost += d > 1 ? 100. + 20. * nt : store;
-          if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0}; }
+          if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0, false}; }
         }
       }
     }
   }
   return best;
+}
+
+bool is_direct(const tetris_fp4_filter *f, int64_t rows, const Geometry &g) {
+  const int64_t tiles = ((g.rows_m ? rows : f->out_channel) + kM - 1) / kM * (((g.rows_m ? f->out_channel : rows) + g.nt - 1) / g.nt);
+  if (g.nt > (g.rows_m ? 128 : 64) || tiles * g.d > (g.half ? 2 : 1) * f->sm_count) return false;  // (one tile per CTA)
+  const Units u = units_of(f->in_channel, std::min<int64_t>(rows, g.rows_m ? kM : g.nt));
+  const int steps = ((f->in_channel + kStep - 1) / kStep + g.d - 1) / g.d;
+  return ((int64_t)steps << u.log) <= kDirectUnits * kStoreWarps;
+}
+
+// The estimate takes the host 0.3 us, so the filter keeps it for the last few numbers of rows.
+Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
+  std::atomic<uint64_t> &kept = f->plans[rows & 7];
+  const uint64_t k = kept.load(std::memory_order_relaxed);
+  if (k >> 24 == (uint64_t)rows) return {(k & 1) != 0, (int)(k >> 8 & 0x1FF), 1 << (k >> 4 & 3), (k & 2) != 0, (k & 4) != 0};
+  Geometry g = estimate(f, rows);
+  g.direct = is_direct(f, rows, g);
+  int d_log = 0;
+  while (1 << d_log < g.d) ++d_log;
+  kept.store((uint64_t)rows << 24 | (uint64_t)g.nt << 8 | (uint64_t)d_log << 4 | (g.direct ? 4 : 0) | (g.half ? 2 : 0) | (g.rows_m ? 1 : 0), std::memory_order_relaxed);
+  return g;
 }
 
 template <int FMT, typename T, bool ROWS_M, bool DIRECT>
@@ -793,14 +815,7 @@ int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const voi
 
 }  // namespace
 
-bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows) {
-  const Geometry g = choose(f, rows);
-  const int64_t tiles = ((g.rows_m ? rows : f->out_channel) + kM - 1) / kM * (((g.rows_m ? f->out_channel : rows) + g.nt - 1) / g.nt);
-  if (g.nt > (g.rows_m ? 128 : 64) || tiles * g.d > (g.half ? 2 : 1) * f->sm_count) return false;  // (one tile per CTA)
-  const Units u = units_of(f->in_channel, std::min<int64_t>(rows, g.rows_m ? kM : g.nt));
-  const int steps = ((f->in_channel + kStep - 1) / kStep + g.d - 1) / g.d;
-  return ((int64_t)steps << u.log) <= kDirectUnits * kStoreWarps;
-}
+bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows) { return choose(f, rows).direct; }
 
 int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
                        int relu, cudaStream_t st) {
