@@ -40,36 +40,47 @@ __device__ __forceinline__ float e4m3_value(uint8_t b) {
   return __half2float(__ushort_as_half((unsigned short)(r & 0xFFFF)));
 }
 
-// The values of a thread's part of a block become quotients by the block's scale; returns the scale's byte.
-template <int FMT, int N>
-__device__ __forceinline__ uint8_t scale_block(float (&v)[N], float top, float tensor_scale, float sixth, float sixth_rest) {
-  if (!(top < __int_as_float(0x7F800000))) {  // codes of 1: the block is NaN whatever it meets
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 1.f;
-    return FMT == TETRIS_FP4_NV ? 0x7F : 0xFF;
-  }
+// A block's scale, from its largest |x|.
+struct BlockScale {
+  uint8_t byte;
+  bool bad;                // an infinity or a NaN is in it: codes of 1, the block is NaN whatever it meets
+  bool far;                // far above what the exponent holds: x / s could leave FP32, the values are brought near first
+  float r, rest, most;     // x / s = x r + x rest; `far`: the largest |x| that makes a difference
+};
+template <int FMT> __device__ __forceinline__ BlockScale block_scale(float top, float tensor_scale, float sixth, float sixth_rest) {
+  BlockScale b;
+  b.bad = !(top < __int_as_float(0x7F800000));
+  b.far = false;
+  b.rest = b.most = 0.f;
   if (FMT == TETRIS_FP4_MX) {
     const int byte = max((int)(__float_as_uint(top) >> 23) - 2, 0);  // at most 252
-    const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= inv;
-    return (uint8_t)byte;
+    b.r = __uint_as_float((uint32_t)(254 - byte) << 23);
+    b.byte = b.bad ? 0xFF : (uint8_t)byte;
+    return b;
   }
   const float within = fminf(top, 4096.f * tensor_scale);  // (beyond 2688 the scale stays at its largest)
-  const uint8_t byte = e4m3_of(__fmaf_rn(within, sixth, within * sixth_rest));
-  const float s = e4m3_value(byte) * tensor_scale;
-  if (top > 1e3f * s && s > 0.f) {  // far above what the exponent holds: x / s could leave FP32
-    const float most = 1e3f * s;
+  b.byte = e4m3_of(__fmaf_rn(within, sixth, within * sixth_rest));
+  const float s = e4m3_value(b.byte) * tensor_scale;
+  b.most = 1e3f * s;
+  b.far = top > b.most && s > 0.f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b.r) : "f"(s));
+  if (s == 0.f) b.r = 0.f;
+  b.rest = __fmaf_rn(-b.r, s, 1.f) * b.r;
+  if (b.bad) b.byte = 0x7F;
+  return b;
+}
+
+// Codes of 8 values of a block.
+template <int FMT> __device__ __forceinline__ uint32_t block_codes(const float *v, const BlockScale &b) {
+  float q[8];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -most), most);
-  }
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  if (s == 0.f) r = 0.f;
-  const float rest = __fmaf_rn(-r, s, 1.f) * r;
+  for (int i = 0; i < 8; ++i) q[i] = FMT == TETRIS_FP4_NV ? __fmaf_rn(v[i], b.r, v[i] * b.rest) : v[i] * b.r;
+  const uint32_t c = codes_of(q);
+  return b.bad ? 0x22222222u : c;
+}
+template <int N> __device__ __forceinline__ void bring_near(float (&v)[N], const BlockScale &b) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __fmaf_rn(v[i], r, v[i] * rest);
-  return byte;
+  for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -b.most), b.most);
 }
 
 }  // namespace tetris

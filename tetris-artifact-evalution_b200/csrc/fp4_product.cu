@@ -38,6 +38,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "fp4.h"
 #include "fp4_block.h"
@@ -411,68 +412,78 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       }
     }
   }
-  // DIRECT: the storing warps quantise the rows r0, ... of a tile.  Unit u: 32 >> (5 - lx) lanes' rows of K step
-  // u >> unit_log; warp w takes units w, w + 8, ..., four at a time so that their loads overlap, a lane 8 values.  Every
-  // warp enters every step, waits for its stage and arrives once it is done with it: a wait for a barrier's phase by its
-  // parity only means something to who has seen the phase before.
+  // DIRECT: the storing warps quantise the rows r0, ... of a tile, K step by K step.  A unit is the lanes' share of 32 >> lx
+  // rows; the warps take the units of a step in turn, several at a time so that their loads and instructions overlap, a
+  // lane 8 values.  Every warp enters every step, waits for its stage and arrives once it is done with it: a wait for a
+  // barrier's phase by its parity only means something to who has seen the phase before.
   int c_stage = 0;
   uint32_t c_parity = 1;
   bool c_withhold = p.withhold_first_load && warp == kFirstStore;
   auto convert = [&](int r0) {
-    constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8, kAtOnce = 4;
-    const int extent = ROWS_M ? p.m_extent : p.n_extent, units = (step1 - step0) << p.unit_log;
-    const int lane_col = lane & ((1 << p.lx) - 1), lane_row = lane >> p.lx, unit_rows = 5 - p.lx;
-    int step = 0;
-    mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
-    auto leave = [&]() {  // this warp is done with the step
+    constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8;
+    const int extent = ROWS_M ? p.m_extent : p.n_extent, units = 1 << p.unit_log, me = warp - kFirstStore;
+    const int lane_col = lane & ((1 << p.lx) - 1), lane_row = lane >> p.lx, blk = lane_col / kLanes;
+    auto some = [&](auto many, int step, int u0) {  // units u0, u0 + 8, ... of the step
+      constexpr int kAtOnce = decltype(many)::value;
+      const int col = step * kStep + lane_col * 8, left = p.K - col;
+      const uint32_t keep = left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u;
+      float v[kAtOnce][8];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int u = u0 + q * kStoreWarps, row = r0 + (u << (5 - p.lx)) + lane_row;
+        int64_t from = row;
+        if (p.px.S > 1) {
+          const uint32_t y = fp4_quot((uint32_t)row, p.by_OW), ox = (uint32_t)row - y * p.px.OW, n = fp4_quot(y, p.by_OH), oy = y - n * p.px.OH;
+          from = ((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S;
+        }
+        load8(p, from * p.x_ld + col, u < units && row < extent ? left : 0, v[q]);
+      }
+      BlockScale b[kAtOnce];
+      bool far = false;
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[q][k]) & 0x7FFFFFFFu);  // (as integers: NaN last)
+#pragma unroll
+        for (int l = 1; l < kLanes; l *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, l));
+        b[q] = block_scale<FMT>(__uint_as_float(top), p.tensor_scale, p.sixth, p.sixth_rest);
+        far |= b[q].far;
+      }
+      if (far) {
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q)
+          if (b[q].far) bring_near(v[q], b[q]);
+      }
+      unsigned char *at = ring + (size_t)c_stage * p.stage_bytes;
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const int u = u0 + q * kStoreWarps, row = (u << (5 - p.lx)) + lane_row;
+        const uint32_t codes = block_codes<FMT>(v[q], b[q]) & keep;
+        if (u < units) {
+          *reinterpret_cast<uint32_t *>(at + (ROWS_M ? 0 : p.n_at) + row * 128 + (((lane_col >> 2) ^ (row & 7)) << 4) + (lane_col & 3) * 4) = codes;
+          if (lane_col % kLanes == 0) at[(ROWS_M ? p.sm_at : p.sn_at) + (blk >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (blk & 3)] = b[q].byte;
+        }
+      }
+    };
+#pragma unroll 1
+    for (int step = step0, turn = me; step < step1; ++step) {
+      mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
+      __syncwarp();
+      if (units <= kStoreWarps) {  // (another warp begins each step)
+        if (turn < units) some(std::integral_constant<int, 1>(), step, turn);
+        turn = (turn - units) & (kStoreWarps - 1);
+      } else {
+#pragma unroll 1
+        for (int u = me; u < units; u += 4 * kStoreWarps) some(std::integral_constant<int, 4>(), step, u);
+      }
       // (the writes went through the generic proxy, the tensor core reads through the async proxy)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0 && !c_withhold) mbar_arrive(bar_full(c_stage));
       c_withhold = false;
       if (++c_stage == p.stages) { c_stage = 0; c_parity ^= 1; }
-    };
-#pragma unroll 1
-    for (int u0 = warp - kFirstStore; u0 < units; u0 += kStoreWarps * kAtOnce) {
-      float v[kAtOnce][8];
-#pragma unroll
-      for (int q = 0; q < kAtOnce; ++q) {
-        const int u = u0 + q * kStoreWarps, row = r0 + ((u & ((1 << p.unit_log) - 1)) << unit_rows) + lane_row;
-        const int col = (step0 + (u >> p.unit_log)) * kStep + lane_col * 8;
-        int64_t from = row;
-        if (p.px.S > 1) {
-          const uint32_t y = fp4_quot((uint32_t)row, p.by_OW), ox = (uint32_t)row - y * p.px.OW, n = fp4_quot(y, p.by_OH), oy = y - n * p.px.OH;
-          from = ((int64_t)n * p.px.H + (int64_t)oy * p.px.S) * p.px.W + (int64_t)ox * p.px.S;
-        }
-        load8(p, from * p.x_ld + col, u < units && row < extent ? p.K - col : 0, v[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < kAtOnce; ++q) {
-        const int u = u0 + q * kStoreWarps;
-        if (u >= units) break;
-        for (; step < u >> p.unit_log; ++step) {
-          leave();
-          mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
-        }
-        __syncwarp();
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[q][k]) & 0x7FFFFFFFu);  // (as integers: NaN last)
-#pragma unroll
-        for (int l = 1; l < kLanes; l *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, l));
-        const uint8_t byte = scale_block<FMT>(v[q], __uint_as_float(top), p.tensor_scale, p.sixth, p.sixth_rest);
-        const int row = ((u & ((1 << p.unit_log) - 1)) << unit_rows) + lane_row, left = p.K - (step0 + step) * kStep - lane_col * 8, blk = lane_col / kLanes;
-        const uint32_t codes = codes_of(v[q]) & (left >= 8 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (4 * left)) - 1u);
-        unsigned char *at = ring + (size_t)c_stage * p.stage_bytes;
-        *reinterpret_cast<uint32_t *>(at + (ROWS_M ? 0 : p.n_at) + row * 128 + (((lane_col >> 2) ^ (row & 7)) << 4) + (lane_col & 3) * 4) = codes;
-        if (lane_col % kLanes == 0) at[(ROWS_M ? p.sm_at : p.sn_at) + (blk >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (blk & 3)] = byte;
-      }
     }
-    for (; step < step1 - step0 - 1; ++step) {
-      leave();
-      mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
-    }
-    leave();
   };
   if (warp < kFirstStore) {
   } else if (p.d == 1) {

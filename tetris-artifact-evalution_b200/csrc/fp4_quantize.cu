@@ -164,16 +164,17 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeParams
     for (int s = 1; s < kLanes; s *= 2) top = Piece<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, s));
     float v[kValues];
     in[u].values(v);
-    const uint8_t byte = scale_block<FMT>(v, Piece<T>::number(top), p.tensor_scale, p.sixth, p.sixth_rest);
-    const uint32_t c = codes_of(v) & keep0;
+    const BlockScale b = block_scale<FMT>(Piece<T>::number(top), p.tensor_scale, p.sixth, p.sixth_rest);
+    if (b.far) bring_near(v, b);
+    const uint32_t c = block_codes<FMT>(v, b) & keep0;
     if (row >= p.rows) continue;
     if (has_codes) {
-      if (kValues == 16) *reinterpret_cast<uint2 *>(codes + row * p.pitch) = make_uint2(c, codes_of(v + kValues - 8) & keep1);
+      if (kValues == 16) *reinterpret_cast<uint2 *>(codes + row * p.pitch) = make_uint2(c, block_codes<FMT>(v + kValues - 8, b) & keep1);
       else *reinterpret_cast<uint32_t *>(codes + row * p.pitch) = c;
     }
     if (has_scale) {
       uint8_t *s = scales + (int64_t)(row >> 7) * p.tiles * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4;
-      *s = byte;
+      *s = b.byte;
       for (int k = 1; k <= fill; ++k) s[k] = 0;
     }
   }
