@@ -14,8 +14,8 @@
 //   Many rows: the rows, D[row][oc].  A lane then holds neighbouring values of its row; a warp stages 32 rows x 128
 //   bytes, which leave as whole lines through a TMA store (each lane storing its own 32 bytes: 3.5 TB/s against 4.9).
 // Roles:
-//   * warp 0 (one thread): per K step of 256 TMA loads of the tile's codes (128 bytes a row, 128-byte swizzle,
-//     zeros past both ends) and bulk copies of the scales, into one ring;
+//   * warp 0 (one thread): per K step of 256 TMA loads of the tile's codes (rows of 128 bytes, or 64 or 32 where K ends
+//     there, swizzled over as much, zeros past both ends) and bulk copies of the scales, into one ring;
 //   * warp 1 (one elected lane): scales from shared into tensor memory (tcgen05.cp), then 4 MMAs;
 //   * eight storing warps: accumulator -> scale, bias, ReLU -> output, beside the next tile's MMAs.
 // Rows that are not quantised yet (DIRECT): before the storing warps store a tile they turn its rows into codes and
@@ -47,7 +47,7 @@ namespace tetris {
 namespace {
 
 constexpr int kM = 128;                  // lanes of a tile
-constexpr int kStep = 256;               // K values of a step: 128 bytes of codes
+constexpr int kStep = 256;               // K values of a step: 128 bytes of codes (one step of 64 or 32 where K is at most 128 or 64)
 constexpr int kStoreWarps = 8, kFirstStore = 2, kThreads = 32 * (kFirstStore + kStoreWarps);
 constexpr int kStagesMax = 8, kSlotsMax = 8;
 constexpr int kBars = 2 * kStagesMax + 8;
@@ -66,6 +66,8 @@ struct ProductParams {
   int m_extent, n_extent;  // rows and channels, or channels and rows
   int m_blocks, n_blocks;  // 128-row blocks of either side's scales
   int steps, last_mmas;    // K steps; MMAs of the last one
+  int row_log;             // log2 of the bytes of a row in a stage
+  uint32_t codes_high;     // high word of the codes' descriptors
   int tiles_k;             // scale tiles of a 128-row block
   int nt;                  // N of the MMAs
   int m_tiles, n_tiles, group;  // tiles; M tiles that are walked side by side
@@ -146,8 +148,8 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // Descriptors of shared memory, low word; the high words are constants.
-// K-major codes in 128-byte rows with the 128-byte swizzle, 8-row groups 1024 bytes apart
-constexpr uint32_t kCodesHigh = 64u | (1u << 14) | (2u << 29);
+// K-major codes in rows of 128, 64 or 32 bytes swizzled over as much, 8-row groups together
+__host__ __device__ constexpr uint32_t codes_high(int row_log) { return (8u << row_log >> 4) | (1u << 14) | ((row_log == 7 ? 2u : row_log == 6 ? 4u : 6u) << 29); }
 // a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart
 constexpr uint32_t kScalesHigh = 8u | (1u << 14);
 __device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | (1u << 16); }
@@ -156,11 +158,11 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t desc) {
   asm volatile("{\n.reg .b64 d;\nmov.b64 d, {%1, %2};\ntcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n}" ::"r"(taddr), "r"(desc), "n"(kScalesHigh) : "memory");
 }
 template <int FMT>
-__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint32_t da, uint32_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+__device__ __forceinline__ void umma_fp4(uint32_t tmem_d, uint32_t da, uint32_t db, uint32_t high, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
 #define TETRIS_FP4_MMA(KIND)                                                                                              \
   asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %7};\nmov.b64 b, {%2, %7};\nsetp.ne.b32 p, %6, 0;\n"  \
                "tcgen05.mma.cta_group::1.kind::" KIND " [%0], a, b, %3, [%4], [%5], p;\n}"                                 \
-               ::"r"(tmem_d), "r"(da), "r"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kCodesHigh) : "memory")
+               ::"r"(tmem_d), "r"(da), "r"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(high) : "memory")
   if (FMT == TETRIS_FP4_NV) TETRIS_FP4_MMA("mxf4nvf4.block_scale.scale_vec::4X");
   else TETRIS_FP4_MMA("mxf4.block_scale.scale_vec::2X");
 #undef TETRIS_FP4_MMA
@@ -297,8 +299,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   };
   auto load_filter = [&](int s, int step) {
     const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-    mbar_expect_tx(bar, DIRECT ? (uint32_t)((ROWS_M ? p.nt : kM) * 128 + scale_tiles(step) * 512)
-                               : (uint32_t)((kM + p.nt) * 128 + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
+    mbar_expect_tx(bar, DIRECT ? (uint32_t)(((ROWS_M ? p.nt : kM) << p.row_log) + scale_tiles(step) * 512)
+                               : (uint32_t)(((kM + p.nt) << p.row_log) + scale_tiles(step) * 512 * (1 + min(rt, p.n_blocks - n0 / 128))));
     if (ROWS_M) load_n(at, bar, step); else load_m(at, bar, step);
   };
   auto load_rows = [&](int s, int step) {
@@ -399,7 +401,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
             if (j < mmas) {
               const int k = FMT == TETRIS_FP4_NV ? j : j >> 1;
               const uint32_t id = FMT == TETRIS_FP4_NV || !(j & 1) ? idesc : idesc | (2u << 4) | (2u << 29);  // (second half of the scale words)
-              umma_fp4<FMT>(acc, at + 2 * j, dn + 2 * j, id, sfm + 4 * k, sfn_row + 4 * rt * k, j == 0 ? more : 1u);
+              umma_fp4<FMT>(acc, at + 2 * j, dn + 2 * j, p.codes_high, id, sfm + 4 * k, sfn_row + 4 * rt * k, j == 0 ? more : 1u);
             }
           }
           umma_commit(bar_empty(s));
@@ -461,7 +463,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         const int u = u0 + q * kStoreWarps, row = (u << (5 - p.lx)) + lane_row;
         const uint32_t codes = block_codes<FMT>(v[q], b[q]) & keep;
         if (u < units) {
-          *reinterpret_cast<uint32_t *>(at + (ROWS_M ? 0 : p.n_at) + row * 128 + (((lane_col >> 2) ^ (row & 7)) << 4) + (lane_col & 3) * 4) = codes;
+          const int swizzle = row >> (7 - p.row_log) & ((1 << (p.row_log - 4)) - 1);
+          *reinterpret_cast<uint32_t *>(at + (ROWS_M ? 0 : p.n_at) + (row << p.row_log) + (((lane_col >> 2) ^ swizzle) << 4) + (lane_col & 3) * 4) = codes;
           if (lane_col % kLanes == 0) at[(ROWS_M ? p.sm_at : p.sn_at) + (blk >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (blk & 3)] = b[q].byte;
         }
       }
@@ -725,6 +728,10 @@ struct Geometry {
   bool direct;             // rows that come as they are: quantised by the product
 };
 
+// Bytes of a row's codes in a stage, as a logarithm: a TMA load takes its time for the zeros behind the last column, too
+// (200704x32x64: 28 us with 128-byte rows).
+int row_log_of(int cols) { return cols <= 64 ? 5 : cols <= 128 ? 6 : 7; }
+
 // The least of an estimate in nanoseconds, whose terms were fitted to 60 shapes (1 to 50000 rows, 64 to 16384
 // columns and channels) in every geometry: its choice takes 1.5 % longer than the best, 15 % at worst.
 //   a K step    the longer of its MMAs and its loads: 51 bytes a nanosecond for half an SM alone, 2 x 40 for two
@@ -737,7 +744,7 @@ struct Geometry {
 //               (1x4096x4096: 4.1 us in 128 halves, 5.5 in 256)
 Geometry estimate(const tetris_fp4_filter *f, int64_t rows) {
   const int steps = (f->in_channel + kStep - 1) / kStep;
-  const double sms = f->sm_count, row_bytes = f->format == TETRIS_FP4_NV ? 144 : 136;  // of a step
+  const double sms = f->sm_count, row_bytes = (1 << row_log_of(f->in_channel)) + (f->format == TETRIS_FP4_NV ? 16 : 8);  // of a step
   Geometry best = {false, 16, 1, true, false};
   double least = 1e300;
   for (int rows_m = 0; rows_m < 2; ++rows_m) {
@@ -812,14 +819,15 @@ int launch(bool rows_m, const CUtensorMap &map_m, const CUtensorMap &map_n, cons
   return rows_m ? launch<FMT, T, true, false>(map_m, map_n, map_y, p, grid, smem, st) : launch<FMT, T, false, false>(map_m, map_n, map_y, p, grid, smem, st);
 }
 
-// A matrix whose rows are `pitch` bytes apart, in boxes of 128 bytes x `box_rows`.
-int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const void *matrix, int64_t cols, int64_t pitch, int64_t rows, int box_rows) {
+// A matrix whose rows are `pitch` bytes apart, in boxes of 2^row_log bytes x `box_rows`, swizzled.
+int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const void *matrix, int64_t cols, int64_t pitch, int64_t rows, int box_rows, int row_log = 7) {
   EncodeFn enc = get_encode();
   if (!enc) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return TETRIS_ERR_UNSUPPORTED; }
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {128u / (cuuint32_t)type_bytes, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {(1u << row_log) / (cuuint32_t)type_bytes, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = row_log == 7 ? CU_TENSOR_MAP_SWIZZLE_128B : row_log == 6 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
   const CUresult r = enc(map, type, 2, const_cast<void *>(matrix), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with code %d", (int)r); return TETRIS_ERR_CUDA; }
   return TETRIS_OK;
 }
@@ -853,8 +861,10 @@ int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t row
   const int64_t total = (int64_t)p.m_tiles * p.n_tiles;
   if (total > 0x3FFFFFFF) { set_error("a product of %lld tiles is outside what the kernels cover", (long long)total); return TETRIS_ERR_UNSUPPORTED; }
   p.total_tiles = (int)total;
-  p.n_at = kM * 128;
-  p.sm_at = p.n_at + g.nt * 128;
+  p.row_log = row_log_of(f->in_channel);
+  p.codes_high = codes_high(p.row_log);
+  p.n_at = kM << p.row_log;
+  p.sm_at = p.n_at + (g.nt << p.row_log);
   p.sn_at = p.sm_at + kt * 512;
   p.stage_bytes = (p.sn_at + rt * kt * 512 + 1023) / 1024 * 1024;
   p.staging = !g.rows_m ? 0 : rt == 2 || g.half ? 1 : 2;
@@ -889,8 +899,8 @@ int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t row
   p.withhold_first_load = test_injection(&p.spin_limit);
   CUtensorMap map_w, map_a = {}, map_y = {};
   int rc;
-  if ((rc = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, f->d_codes, f->pitch, f->pitch, f->out_channel, g.rows_m ? g.nt : kM)) ||
-      (!direct && (rc = encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, f->pitch, f->pitch, rows, g.rows_m ? kM : g.nt))) ||
+  if ((rc = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, f->d_codes, f->pitch, f->pitch, f->out_channel, g.rows_m ? g.nt : kM, p.row_log)) ||
+      (!direct && (rc = encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, f->pitch, f->pitch, rows, g.rows_m ? kM : g.nt, p.row_log))) ||
       (p.tma_store && (rc = encode(&map_y, y_type == TETRIS_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, bytes, y,
                                    f->out_channel, ld * bytes, rows, 32))))
     return rc;
