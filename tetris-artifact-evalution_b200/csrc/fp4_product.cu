@@ -5,8 +5,8 @@
 //
 // What bounds it: large products the tensor cores and the card's power (4096x4096x16384, MX: 3.8 to 4.2 PFLOP/s at
 // 1.6 to 1.9 GHz and 1000 W; the MMAs alone, without loads and copies of scales, 5.5); few rows the reading of the
-// filter (16x8192x8192, NV: 9.4 us, 4.1 TB/s); layers with few columns the writing of the output (50176x64x256: 12.1 us,
-// 4.4 TB/s); small products the launch (1x2048x1000: 3 us).
+// filter (16x8192x8192, NV: 9.4 us, 4.1 TB/s); layers with few columns the writing of the output (50176x64x256: 11.1 us,
+// 4.8 TB/s); small products the launch (1x2048x1000: 3 us).
 //
 // Which operand is on the M side (128 lanes of tensor memory) depends on the number of rows.
 //   Few rows: the filter, D[oc][row].  16 to 64 rows cost a narrow N instead of an empty M; a lane is a channel,
@@ -476,6 +476,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       if (units <= kStoreWarps) {  // (another warp begins each step)
         if (turn < units) some(std::integral_constant<int, 1>(), step, turn);
         turn = (turn - units) & (kStoreWarps - 1);
+      } else if (units == 2 * kStoreWarps) {
+        some(std::integral_constant<int, 2>(), step, me);
       } else {
 #pragma unroll 1
         for (int u = me; u < units; u += 4 * kStoreWarps) some(std::integral_constant<int, 4>(), step, u);
@@ -705,10 +707,10 @@ EncodeFn get_encode() {
 constexpr size_t kSmemMost = 227 * 1024, kSmemHalf = 113 * 1024;   // (1 KB of either goes into the ring's alignment)
 constexpr size_t kSmemLeast = 117 * 1024;
 
-// A product quantises its rows itself where a storing warp has at most this many units of it to do.  A unit takes such a
-// warp about 0.5 us, which the filter's loads hide in part; a launch of its own takes 2 us of the device, in part hidden,
-// too, and 2.2 us of the host (16x1024x1024, 2 units: 4.8 us on the device and 6.3 on the host in one launch, 4.4 and
-// 8.6 in two; 16x8192x8192, 16 units: 19 and 10 us on the device).
+// A product quantises its rows itself where a storing warp has at most this many units of it to do.  Up to there it takes
+// no longer than a launch of its own before the product, and the host has one launch less, 2.2 us (16x1024x1024, 2 units:
+// 4.1 us on the device in one launch, 4.5 in two; 22x832x32, 4 units: 5.2 and 4.5; 51x1824x640, 8 units: 7.5 and 5.8;
+// 16x8192x8192, 16 units: 18 and 10.7).
 constexpr int kDirectUnits = 4;
 
 // How the rows of a tile are cut into units of a warp: 2^lx lanes take a row's part of a K step.
