@@ -4,8 +4,8 @@
 //
 // Bound: HBM; what stands in its way is the number of instructions, so a thread keeps one column position and walks
 // down a few rows, takes 32 bytes at a time, and finds the largest one of 16-bit types as packed integers.  4096 x 8192
-// (floors at 6.55 TB/s in brackets): from FP32 23.4 us MX, 25.0 NV (23.3), from BF16 16.9 and 18.8 (13.0); back to
-// FP32 25.1 (23.3), to BF16 14.9 (13.0).
+// (floors at 6.55 TB/s in brackets): from FP32 23.2 us MX, 23.9 NV (23.3), from BF16 15.2 and 17.9 (13.0); back to
+// FP32 25.0 (23.3), to BF16 14.8 (13.0).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
