@@ -102,6 +102,29 @@ def test_host_tensors_are_checked_before_the_call(tb):
         tb.fp4_quantize(x, buf, buf, 4, 64, tb.FP4_MX, dtype=tb.BF16)
 
 
+def test_numbers_that_do_not_fit_the_calls_integers(tb):
+    """A number of 33 bits would reach the library as another one, a stride of 2^32 + 1 as one that writes every pixel."""
+    import types
+    import torch
+    wide, f = (1 << 32) + 1, types.SimpleNamespace(in_channel_=32, out_channel_=8, format_=tb.FP4_NV, handle=None, _handle=None)
+    x, y, buf = torch.zeros(4, 32), torch.zeros(4, 8), torch.zeros(4096, dtype=torch.uint8)
+    calls = [lambda: tb.fp4_sizes(1, wide, tb.FP4_MX),
+             lambda: tb.fp4_quantize(4096, 4096, 4096, 1, wide, tb.FP4_MX),
+             lambda: tb.fp4_dequantize(4096, 4096, 4096, 1, wide, tb.FP4_MX),
+             lambda: tb.fp4_quantize(x, buf, buf, 4, 32, tb.FP4_NV, exponent=wide),
+             lambda: tb.fp4_dequantize(buf, buf, x, 4, 32, tb.FP4_NV, exponent=-wide),
+             lambda: tb.fp4_product(f, buf, buf, y, 4, exponent=wide),
+             lambda: tb.fp4_linear(f, x, y, 4, exponent=wide),
+             lambda: tb.fp4_conv2d(f, x, y, 1, 2, 2, wide, 0),
+             lambda: tb.fp4_conv2d(f, x, y, 1, 2, 2, 1, wide - 1),
+             lambda: tb.fp4_conv2d(f, 4096, 4096, wide, 2, 2, 1, 0),
+             lambda: tb.fp4_conv2d(f, x, y, 1, 2, 2, 1, 0, exponent=wide),
+             lambda: tb.Fp4Filter(np.zeros((8, 32), np.float32), 32, 8, format=tb.FP4_NV, exponent=wide)]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_reference_rounds_to_even_and_saturates():
     v = np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, -0.25, -5.0] + [0] * 22])
     code, byte = ref.quantize(v, ref.MX)

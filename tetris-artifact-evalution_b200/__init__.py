@@ -441,6 +441,13 @@ _FP4_TYPES = {"torch.float32": FP32, "torch.bfloat16": BF16, "torch.float16": FP
 _fp4_type_of = {}                 # torch dtype -> type, filled as dtypes are met
 
 
+def _fp4_ints(*values):
+    """Numbers that the calls take in 32 bits: a longer one would arrive as another one."""
+    for v in values:
+        if not -0x80000000 <= v <= 0x7FFFFFFF:
+            raise ValueError("%d does not fit 32 bits" % v)
+
+
 def _fp4_type(x, dtype, what):
     """The type of a dense argument: `dtype` for an address, the tensor's own for a tensor."""
     if type(x) is int:
@@ -505,6 +512,7 @@ def _fp4_storage(rows, cols, format):
 
 def fp4_sizes(rows, cols, format):
     """(bytes of the codes, bytes of the scales) of a rows x cols matrix in 4 bits."""
+    _fp4_ints(cols, format)
     c, s = ctypes.c_int64(0), ctypes.c_int64(0)
     _check(lib().tetris_fp4_sizes(rows, cols, format, None, ctypes.byref(c), ctypes.byref(s)))
     return c.value, s.value
@@ -513,6 +521,7 @@ def fp4_sizes(rows, cols, format):
 def fp4_quantize(input, codes, scales, rows, cols, format, exponent=0, ld=0, dtype=None, cuda_stream=None):
     """Device `input` (rows x cols, FP32 / BF16 / FP16) -> `codes` and `scales` (uint8 device buffers of
     fp4_sizes bytes), asynchronous.  `exponent`: of the whole tensor, FP4_NV only."""
+    _fp4_ints(cols, format, exponent)
     need = _fp4_storage(rows, cols, format)
     x, ld = _fp4_dense(input, rows, cols, ld, "the input")
     _check(lib().tetris_fp4_quantize(x, _fp4_type(input, dtype, "the input"), rows, cols, ld, format, exponent,
@@ -522,6 +531,7 @@ def fp4_quantize(input, codes, scales, rows, cols, format, exponent=0, ld=0, dty
 
 def fp4_dequantize(codes, scales, output, rows, cols, format, exponent=0, ld=0, dtype=None, cuda_stream=None):
     """The values that `codes` and `scales` stand for, into device `output` (rows x cols), asynchronous."""
+    _fp4_ints(cols, format, exponent)
     need = _fp4_storage(rows, cols, format)
     y, ld = _fp4_dense(output, rows, cols, ld, "the output")
     _check(lib().tetris_fp4_dequantize(_fp4_bytes(codes, need[0], "codes"), _fp4_bytes(scales, need[1], "scales"), rows, cols,
@@ -540,6 +550,7 @@ class Fp4Filter:
     def __init__(self, filter, in_channel, out_channel, kernel_size=1, format=FP4_MX, exponent=FP4_EXPONENT_AUTO, device=None,
                  cuda_stream=None):
         self._handle = _VP()
+        _fp4_ints(in_channel, out_channel, kernel_size, format, exponent, device or 0)
         if hasattr(filter, "data_ptr"):
             if not filter.is_contiguous():
                 raise ValueError("the filter has to be contiguous")
@@ -596,6 +607,7 @@ def fp4_product(fp4_filter, codes, scales, output, rows, exponent=0, bias=None, 
     """`output` (device, rows x out_channel) = quantised activations times the filter (+ bias, ReLU),
     asynchronous; `codes` and `scales` as fp4_quantize writes them in the filter's format."""
     f = fp4_filter
+    _fp4_ints(exponent)
     need = _fp4_storage(rows, f.in_channel_, f.format_)
     y, ld = _fp4_dense(output, rows, f.out_channel_, ld, "the output")
     status = (_lib or lib()).tetris_fp4_product(
@@ -630,6 +642,7 @@ def fp4_linear(fp4_filter, input, output, rows, workspace=None, exponent=0, bias
     times the filter (+ bias, ReLU), asynchronous.  `workspace`: fp4_workspace bytes on the device."""
     f = fp4_filter
     n = f.out_channel_
+    _fp4_ints(exponent)
     x, ld_input = _fp4_dense(input, rows, f.in_channel_, ld_input, "the input")
     y, ld_output = _fp4_dense(output, rows, n, ld_output, "the output")
     room, size = _fp4_room(workspace)
@@ -645,6 +658,7 @@ def fp4_conv2d(fp4_filter, input, output, batch_size, img_h, img_w, stride, padd
                relu=False, cuda_stream=None):
     """The 1x1 layer with a 4-bit filter: device NHWC FP32 in and out as sparse_conv2d, padding 0."""
     f = fp4_filter
+    _fp4_ints(batch_size, img_h, img_w, stride, padding, exponent)
     pixels = batch_size * ((img_h - 1) // stride + 1) * ((img_w - 1) // stride + 1) if stride > 0 else 0
     if _fp4_type(input, None, "the input") != FP32 or _fp4_type(output, None, "the output") != FP32:
         raise ValueError("a 4-bit layer takes and gives float32")
