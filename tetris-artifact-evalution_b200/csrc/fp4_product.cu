@@ -685,7 +685,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     if (tid == 0) atomicExch(p.error_flag, 1);
     __syncwarp();
   }
-  if (p.d > 1) cluster_wait();  // (no CTA leaves while another one may still push into it)
+  if (p.d > 1) {
+    cluster_wait();  // (no CTA leaves while another one may still push into it)
+    if (tid == 0 && *abort_flag) mbar_drain(bar_sums(), 0);  // (one that gave up did not wait for what the others sent)
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
 }
 
