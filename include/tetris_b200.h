@@ -425,8 +425,8 @@ unsigned long long tetris_launch_count(void);
  * kernel raises a flag, lets every role drain (loads, copies and MMAs already started are waited
  * for), frees its tensor memory and returns, and tetris_filter_check reports TETRIS_ERR_CUDA once.
  * tetris_test_inject(TETRIS_INJECT_WITHHOLD_LOAD, n) makes the following tensor-core launches of
- * this process leave out every CTA's first activation load and give up after n polls (0: the
- * built-in limit, seconds), so that a test can see that path end to end without a GPU fault: the
+ * this process leave out every CTA's first activation load (4-bit products: all loads of its first
+ * K step) and give up after n polls (0: the built-in limit, seconds), so that a test can see that path end to end without a GPU fault: the
  * launch returns normally, its output is unspecified, the context stays usable.
  * tetris_test_inject(TETRIS_INJECT_NONE, 0) switches it off.  Never use it outside tests.
  */

@@ -541,6 +541,35 @@ def test_bounded_wait_gives_up_and_the_next_product_passes(tb, torch_cuda, rows)
     check_product(y, want, terms, k, torch)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(3000, 4096, 4096), (300, 8192, 200), (40, 16384, 300), (1, 16384, 200), (1, 8192, 20000), (2, 8192, 9000)])
+def test_give_up_where_stages_are_used_again(tb, torch_cuda, fmt, rows, k, n):
+    """More K steps than the ring has stages: after a wait that gave up nothing may be sent for into a stage whose
+    last load is still owed, and the product that follows at once, placed while the first one ends, is right.
+    Many tiles of a CTA, clusters, rows quantised by the product itself."""
+    torch = torch_cuda
+    x = activations(torch, rows, k, 33, spread=1.0, dtype="bf16")
+    f, w = filter_and_weights(tb, torch, n, k, fmt, 34)
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    want, y, z = (torch.empty(rows, n, device="cuda") for _ in range(3))
+    tb.fp4_linear(f, x, want, rows, work)
+    f.check()
+    for _ in range(3):
+        z.fill_(float("nan"))
+        torch.cuda.synchronize()
+        tb.test_inject(1, 500)
+        try:
+            tb.fp4_linear(f, x, y, rows, work)
+        finally:
+            tb.test_inject(0)
+        tb.fp4_linear(f, x, z, rows, work)
+        with pytest.raises(tb.TetrisError) as e:
+            f.check()
+        assert e.value.status == 2 and "gave up" in str(e.value)
+        assert torch.equal(z, want)
+    f.check()
+
+
 def test_offsets_past_32_bits(tb, torch_cuda):
     """17 GB of activations, 4.3 GB of codes: the last rows come out as they do on their own."""
     torch = torch_cuda

@@ -27,8 +27,10 @@
 // Few tiles: the K range is cut over a cluster of up to 8 CTAs, whose sums are copied into the shared memory of the
 // CTA that owns a column (one bulk copy per owner, counted on its barrier) and added in slice order: bit-reproducible,
 // no workspace.
-// Every barrier wait is bounded; on a timeout an error flag is raised, all roles drain, tensor memory is
-// freed and the kernel returns; tetris_fp4_filter_check reports it.
+// Every barrier wait is bounded; on a timeout an error flag is raised, all roles stop, what the CTA has in flight lands,
+// tensor memory is freed and the kernel returns; tetris_fp4_filter_check reports it.  A role whose wait gave up neither
+// arrives at nor commits to a barrier again: a stage is then never sent for while its last phase is open, and the phases
+// that the end of the kernel waits for are those of the loads in flight.
 // Tried and dropped: pairs of CTAs on a tile of 256 x 256 (cta_group::2, each stage's arrival passed on to the CTA that
 // issues: 173 us for 4096x4096x16384 against 138), scales copied a step ahead of the MMAs (181), warps of their own that
 // quantise rows of large layers (50176x64x256 15.5 us against 19.4 in two launches, 12544x256x512 20.1 against 12.5).
@@ -262,7 +264,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   float *bias_rows = reinterpret_cast<float *>(staging + (p.d > 1 ? p.nt * kSumPitch * 4 : kStoreWarps * kStageOut * p.staging));
   uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(bias_rows) + kBiasBytes);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);  // a wait gave up; polls of a wait; K steps sent for
   // (the warp number as a value that is the same in all lanes for the compiler, too: what the tensor core is told
   // can then be worked out in uniform registers; 4096x4096x16384 147 -> 144 us)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -305,7 +307,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   };
   auto load_rows = [&](int s, int step) {
     const uint32_t at = smem_u32(ring + (size_t)s * p.stage_bytes), bar = bar_full(s);
-    if (loads++ == 0 && p.withhold_first_load) return;  // (test: that step never arrives, its reader gives up)
+    if (loads++ == 0 && p.withhold_first_load) return;
     if (DIRECT) return;
     if (ROWS_M) load_m(at, bar, step); else load_n(at, bar, step);
   };
@@ -321,7 +323,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     // the filter's part of the empty ring is sent for while the launch before this one drains
     decode(p, tile0, m0, n0);
-    for (int i = 0; i < ahead; ++i) load_filter(i, step0 + i);
+    for (int i = p.withhold_first_load; i < ahead; ++i) load_filter(i, step0 + i);  // (test: the first step never arrives)
     if (p.d > 1) {
       const int live = min(p.nt, p.n_extent - n0) - (rank << p.per_log);  // columns that this CTA adds up
       mbar_expect_tx(bar_sums(), (uint32_t)(max(0, min(1 << p.per_log, live)) * p.d * kSumPitch * 4));
@@ -354,13 +356,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
           if (++s == p.stages) { s = 0; parity ^= 1; }
         }
       }
+      abort_flag[2] = loads;
     }
   } else if (warp == 1) {
-    // The loop has no early exits: a wait that gave up raises the abort flag, later waits then return at once.
+    // The loop has no early exits: after a wait that gave up it runs dry, without MMAs and commits (what the elected lane
+    // has waited for is what counts).
     constexpr uint32_t kFormats = (1u << 7) | (1u << 10) | (FMT == TETRIS_FP4_NV ? 0u : 1u << 23) | ((uint32_t)(kM >> 4) << 24);
     const uint32_t idesc = kFormats | ((uint32_t)(p.nt >> 3) << 17);
+    bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
+      if (!mbar_try_wait(bar, parity)) ok = ok && mbar_wait(bar, parity, abort_flag);
       __syncwarp();
     };
     const uint32_t ring0 = desc_low(smem_u32(ring)), stage_step = (uint32_t)p.stage_bytes >> 4;
@@ -387,7 +392,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         const int n = min(kTiles, p.tiles_k - step * kTiles), mmas = step == p.steps - 1 ? p.last_mmas : 4;
         const uint32_t dsm = at + (p.sm_at >> 4), dsn = at + (p.sn_at >> 4), dn = at + (p.n_at >> 4);
         const uint32_t more = step > step0;
-        if (elect_one()) {
+        if (elect_one() && ok) {
 #pragma unroll
           for (int k = 0; k < kTiles; ++k) {
             if (k < n) {
@@ -417,10 +422,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   // DIRECT: the storing warps quantise the rows r0, ... of a tile, K step by K step.  A unit is the lanes' share of 32 >> lx
   // rows; the warps take the units of a step in turn, several at a time so that their loads and instructions overlap, a
   // lane 8 values.  Every warp enters every step, waits for its stage and arrives once it is done with it: a wait for a
-  // barrier's phase by its parity only means something to who has seen the phase before.
-  int c_stage = 0;
+  // barrier's phase by its parity only means something to who has seen the phase before.  (After a wait that gave up it
+  // walks on without waiting and arriving: its lanes meet in shuffles.)
+  int c_stage = 0, c_steps = 0x7FFFFFFF;   // c_steps: steps that it was done with when a wait gave up
   uint32_t c_parity = 1;
-  bool c_withhold = p.withhold_first_load && warp == kFirstStore;
+  bool c_ok = true;
   auto convert = [&](int r0) {
     constexpr int kLanes = (FMT == TETRIS_FP4_NV ? 16 : 32) / 8;
     const int extent = ROWS_M ? p.m_extent : p.n_extent, units = 1 << p.unit_log, me = warp - kFirstStore;
@@ -471,7 +477,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     };
 #pragma unroll 1
     for (int step = step0, turn = me; step < step1; ++step) {
-      mbar_wait(bar_empty(c_stage), c_parity, abort_flag);
+      if (!mbar_try_wait(bar_empty(c_stage), c_parity) && !(c_ok && mbar_wait(bar_empty(c_stage), c_parity, abort_flag))) {
+        if (c_ok) c_steps = step - step0;
+        c_ok = false;
+      }
       __syncwarp();
       if (units <= kStoreWarps) {  // (another warp begins each step)
         if (turn < units) some(std::integral_constant<int, 1>(), step, turn);
@@ -485,8 +494,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       // (the writes went through the generic proxy, the tensor core reads through the async proxy)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0 && !c_withhold) mbar_arrive(bar_full(c_stage));
-      c_withhold = false;
+      if (lane == 0 && c_ok) mbar_arrive(bar_full(c_stage));
       if (++c_stage == p.stages) { c_stage = 0; c_parity ^= 1; }
     }
   };
@@ -504,8 +512,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
       const int b = i & acc_log, mq = m0 + quarter * 32, m = mq + lane, n_first = n0;
       const float lane_bias = !ROWS_M && p.bias && m < p.m_extent ? p.bias[m] : 0.f;
       if (DIRECT) convert(ROWS_M ? m0 : n0);
-      if (!mbar_try_wait(bar_pfull(b), (i >> acc_log) & 1)) mbar_wait(bar_pfull(b), (i >> acc_log) & 1, abort_flag);
-      __syncwarp();
+      bool ok = mbar_try_wait(bar_pfull(b), (i >> acc_log) & 1);
+      if (!ok) ok = mbar_wait(bar_pfull(b), (i >> acc_log) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (b ? p.acc1 : 0);
       bool told = !over;
@@ -675,6 +684,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (*abort_flag) {  // what this CTA has in flight must land before it leaves
+    // (stages on their way also wait for the arrivals of quantising warps that stopped before them: at most one each, since
+    // a stage is sent for again only after its last phase)
+    if (DIRECT && warp >= kFirstStore && lane == 0)
+      for (int v = c_steps; v < abort_flag[2]; ++v) mbar_arrive(bar_full(v % p.stages));
     if (tid == 0)
       for (int v = max(loads - p.stages, p.withhold_first_load ? 1 : 0); v < loads; ++v) mbar_drain(bar_full(v % p.stages), (uint32_t)(v / p.stages) & 1u);
     if (warp == 1) {
