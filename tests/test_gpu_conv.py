@@ -554,6 +554,42 @@ def test_bounded_wait_gives_up_and_the_next_launch_passes(tb, torch_cuda, oracle
 
 
 @pytest.mark.parametrize("case", [
+    # (n, ic, h, w, oc, ks, stride): more K steps than the rings have stages: many tiles of a CTA, K ranges cut over
+    # clusters, 1x1 and strided layers, stacked tiles
+    (16, 256, 28, 28, 256, 3, 1), (1, 512, 14, 14, 512, 3, 1), (4, 1024, 14, 14, 256, 1, 1), (4, 128, 56, 56, 128, 3, 2),
+    (8, 512, 28, 28, 64, 1, 1)])
+def test_give_up_where_stages_are_used_again(tb, torch_cuda, case):
+    """After a wait that gave up nothing may be sent for into a stage whose last load is still owed, and the launch
+    that follows at once, placed while the first one ends, is right."""
+    torch = torch_cuda
+    n, ic, h, w, oc, ks, stride = case
+    rng = np.random.default_rng(4243)
+    filt = (rng.standard_normal((oc, ic, ks, ks)) * 0.05 * (rng.random((oc, ic, ks, ks)) >= 0.8)).astype(np.float32)
+    f = tb.SparseFilter(filt, ic, oc, ks)
+    pad, v = ks // 2, VARIANTS["tensor16"]
+    oh, ow = (h - 1) // stride + 1, (w - 1) // stride + 1
+    x = torch.rand(n, h, w, ic, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7))
+    want, y, z = (torch.full((n, oh, ow, oc), float("nan"), device="cuda") for _ in range(3))
+    tb.sparse_conv2d(f, x, want, n, h, w, stride, pad, variant=v)
+    f.check()
+    for _ in range(3):
+        z.fill_(float("nan"))
+        torch.cuda.synchronize()
+        tb.test_inject(1, 500)
+        try:
+            tb.sparse_conv2d(f, x, y, n, h, w, stride, pad, variant=v)
+        finally:
+            tb.test_inject(0)
+        tb.sparse_conv2d(f, x, z, n, h, w, stride, pad, variant=v)
+        with pytest.raises(tb.TetrisError) as err:
+            f.check()
+        assert err.value.status == 2, err.value
+        assert torch.equal(z, want)
+    f.check()
+    f.close()
+
+
+@pytest.mark.parametrize("case", [
     # (n, ic, h, w, oc, ks, pad): 1x1 and short-K layers on images whose tiles take the TMA-store epilogue of the
     # split-TF32 kernel: 128-pixel tiles, tiles that span the image's height, channel counts that end inside a
     # 32-channel box, images that end inside a tile

@@ -157,6 +157,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   *abort_flag = 1;
   return false;
 }
+// The MMA warp's wait once a first poll has failed: after a give-up it returns when warp 0 sends for nothing more.  A call,
+// so that the warp's unrolled loop holds one poll and no loops (56x56 256->256 3x3 batch 16 134 -> 129 us, 14x14 512->512
+// 43.8 -> 41.3; the second wait inlined with the first: 139 and 46.6).
+__device__ __noinline__ void mbar_wait_or_stop(uint32_t bar, uint32_t parity, volatile int *abort_flag, volatile int *loads_over) {
+  if (mbar_wait(bar, parity, abort_flag)) return;
+  for (int i = 0; i < (1 << 16) && !*loads_over; ++i) __nanosleep(64);
+}
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
@@ -321,6 +328,7 @@ conv_tc16_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gtabs + kSumWarps * (NC / 8));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   unsigned *seen_slot = tmem_slot + 3;            // largest |activation| of this CTA, FP32 bits
+  volatile int *loads_over = reinterpret_cast<volatile int *>(tmem_slot + 4);  // warp 0 sends for nothing more (in this pass)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar_xfull = [&](int s) { return smem_u32(&bars[s]); };
   auto bar_xconv = [&](int s) { return smem_u32(&bars[kXStagesMax + s]); };
@@ -339,6 +347,7 @@ conv_tc16_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     abort_flag[0] = 0;
     abort_flag[1] = (int)(p.spin_limit ? p.spin_limit : kSpinLimit);
     *seen_slot = 0u;
+    *loads_over = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
   }
@@ -498,21 +507,24 @@ conv_tc16_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             __nanosleep(20);
           }
         }
+        *loads_over = 1;
       }
     } else if (warp == 1) {
       // ---- MMA issue (converged warp, one elected lane, so that descriptors stay in uniform
       //      registers): per K step one wait, 6 (4) MMAs, one commit ----
       // A K step of the smallest tiles takes the tensor core 200 clocks, about what this warp needs
-      // to wait, issue and commit, so the loop is kept short: no early exits (a wait that gave up
-      // raises the abort flag, later waits then return at once and the loop runs dry), 3x3 taps
-      // unrolled, ring positions counted along.
+      // to wait, issue and commit, so the loop is kept short: no early exits (after a wait that gave up
+      // the loop runs dry), 3x3 taps unrolled, ring positions counted along.  What it then commits says
+      // nothing about a stage, whose last phase may still be open, so it first lets warp 0 stop, which
+      // would send for the stage again.  (MMAs and commits left out instead: 3 to 6 % on large layers;
+      // warp 0 looking at the flag before each load: 1 %.)
       const uint32_t idesc = (1u << 4) | ((uint32_t)(p.npx >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
       const uint32_t sbo_x = (uint32_t)(p.mode == kGrid ? p.PW * 128 : 1024);
       const uint64_t dx0 = smem_desc(smem_u32(xbase), sbo_x, 2), dw0 = smem_desc(smem_u32(wbase), STACK ? 512 : 1024, STACK ? 4 : 2);
       const uint32_t dx_hi = (uint32_t)(dx0 >> 32), dw_hi = (uint32_t)(dw0 >> 32);
       const uint32_t x_step = (uint32_t)(p.x_stage_bytes >> 4), row_step = (uint32_t)(p.PW * 8);
       auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!mbar_try_wait(bar, parity)) mbar_wait(bar, parity, abort_flag);
+        if (!mbar_try_wait(bar, parity)) mbar_wait_or_stop(bar, parity, abort_flag, loads_over);
         __syncwarp();
       };
       int k = 0;                  // K step of the band
@@ -819,7 +831,7 @@ conv_tc16_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     }
     first = false;
     __syncthreads();
-    if (tid == 0) *seen_slot = 0u;
+    if (tid == 0) { *seen_slot = 0u; *loads_over = 0; }
     __syncthreads();
   }
 
