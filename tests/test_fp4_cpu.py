@@ -125,6 +125,32 @@ def test_numbers_that_do_not_fit_the_calls_integers(tb):
             call()
 
 
+def test_numbers_that_do_not_fit_64_bits(tb):
+    """Rows and row distances of 65 bits would arrive as other ones, a type of 33 bits as FP32."""
+    import types
+    import torch
+    wide, f = 1 << 64, types.SimpleNamespace(in_channel_=32, out_channel_=8, format_=tb.FP4_MX, handle=None, _handle=None)
+    few, buf = torch.zeros(10), torch.zeros(4096, dtype=torch.uint8)
+    calls = [lambda: tb.fp4_sizes(wide, 32, tb.FP4_MX),
+             lambda: tb.fp4_workspace(f, wide + 1),
+             lambda: tb.fp4_quantize(4096, 4096, 4096, wide, 32, tb.FP4_MX),
+             lambda: tb.fp4_quantize(4096, 4096, 4096, 0, 32, tb.FP4_MX, ld=wide),
+             lambda: tb.fp4_dequantize(4096, 4096, 4096, -wide, 32, tb.FP4_MX),
+             lambda: tb.fp4_dequantize(4096, 4096, 4096, 0, 32, tb.FP4_MX, ld=-wide),
+             lambda: tb.fp4_quantize(few, buf, buf, 4 - wide, 32, tb.FP4_MX),
+             lambda: tb.fp4_quantize(few, buf, buf, 4, 32, tb.FP4_MX, ld=-wide),
+             lambda: tb.fp4_product(f, 4096, 4096, 4096, wide),
+             lambda: tb.fp4_product(f, 4096, 4096, 4096, 0, ld=wide),
+             lambda: tb.fp4_linear(f, 4096, 4096, wide),
+             lambda: tb.fp4_linear(f, 4096, 4096, 0, ld_input=wide),
+             lambda: tb.fp4_linear(f, 4096, 4096, 0, ld_output=wide),
+             lambda: tb.fp4_quantize(4096, 4096, 4096, 0, 32, tb.FP4_MX, dtype=1 << 32),
+             lambda: tb.fp4_dequantize(4096, 4096, 4096, 0, 32, tb.FP4_MX, dtype=1 << 32)]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_reference_rounds_to_even_and_saturates():
     v = np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, -0.25, -5.0] + [0] * 22])
     code, byte = ref.quantize(v, ref.MX)

@@ -448,10 +448,20 @@ def _fp4_ints(*values):
             raise ValueError("%d does not fit 32 bits" % v)
 
 
+def _fp4_longs(*values):
+    """The same for numbers that the calls take in 64 bits."""
+    for v in values:
+        if not -0x8000000000000000 <= v <= 0x7FFFFFFFFFFFFFFF:
+            raise ValueError("%d does not fit 64 bits" % v)
+
+
 def _fp4_type(x, dtype, what):
     """The type of a dense argument: `dtype` for an address, the tensor's own for a tensor."""
     if type(x) is int:
-        return FP32 if dtype is None else dtype
+        if dtype is None:
+            return FP32
+        _fp4_ints(dtype)
+        return dtype
     t = _fp4_type_of.get(x.dtype)
     if t is not None and dtype is None:
         return t
@@ -469,9 +479,11 @@ def _fp4_dense(x, rows, cols, ld, what):
     """(address, row distance) of a dense device matrix of rows x cols.  A two-dimensional tensor may have
     rows further apart than cols; any other has to be contiguous."""
     if type(x) is int:
+        _fp4_longs(rows, ld)
         return x, ld
     if not ld and x.is_contiguous() and x.numel() == rows * cols:
         return x.data_ptr(), 0
+    _fp4_longs(rows, ld)
     if x.dim() == 2 and x.shape[0] == rows and x.shape[1] == cols:
         apart, step = x.stride()
         if (step != 1 and cols > 1) or (apart < cols and rows > 1):
@@ -513,6 +525,7 @@ def _fp4_storage(rows, cols, format):
 def fp4_sizes(rows, cols, format):
     """(bytes of the codes, bytes of the scales) of a rows x cols matrix in 4 bits."""
     _fp4_ints(cols, format)
+    _fp4_longs(rows)
     c, s = ctypes.c_int64(0), ctypes.c_int64(0)
     _check(lib().tetris_fp4_sizes(rows, cols, format, None, ctypes.byref(c), ctypes.byref(s)))
     return c.value, s.value
@@ -620,6 +633,7 @@ def fp4_product(fp4_filter, codes, scales, output, rows, exponent=0, bias=None, 
 
 def fp4_workspace(fp4_filter, rows):
     """Bytes of device workspace that fp4_linear and fp4_conv2d need for `rows` rows (pixels)."""
+    _fp4_longs(rows)
     n = ctypes.c_int64(0)
     _check(lib().tetris_fp4_workspace(fp4_filter.handle, rows, ctypes.byref(n)))
     return n.value
