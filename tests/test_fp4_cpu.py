@@ -1,6 +1,8 @@
 """CPU: sizes and refusals of the 4-bit entry points (nothing here reaches a kernel), and the host's own
 description of the formats."""
 import ctypes
+import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -156,3 +158,51 @@ def test_reference_rounds_to_even_and_saturates():
     code, byte = ref.quantize(v, ref.MX)
     assert byte[0, 0] == 127 and list(code[0, :10]) == [0, 2, 2, 4, 4, 6, 6, 7, 0, 14]
     assert ref.E4M3[0x7E] == 448 and ref.E4M3[1] == 2.0 ** -9 and np.isnan(ref.E4M3[0x7F])
+
+
+def _to_24_bits(x):
+    """A Fraction rounded to 24 significant bits, ties to even."""
+    if x == 0:
+        return x
+    e = math.frexp(float(abs(x)))[1] - 24
+    unit = Fraction(2) ** e
+    n = x / unit
+    n = n.numerator // n.denominator + (1 if (n % 1, n.numerator // n.denominator % 2) > (Fraction(1, 2), 0) else 0)
+    return n * unit
+
+
+def _neighbours(x):
+    """x of at most 24 bits with the numbers of 24 bits before and behind it."""
+    up = Fraction(2) ** (math.frexp(float(x))[1] - 24)
+    down = up / 2 if math.frexp(float(x))[0] == 0.5 else up
+    return (x - down, -1), (x, 0), (x + up, 1)
+
+
+@pytest.mark.parametrize("m", range(8, 16))
+def test_quotient_of_two_operations_on_and_beside_the_borders(m):
+    """The codes' quotient x / s as x r + x r', r' = r (1 - r s), all in 24 bits, in exact arithmetic: on a border
+    between codes and one last place beside it, it lies where the real quotient does, whichever reciprocal within two
+    last places r is.  It never falls where x grows (x r grows by 2^-24 |x r| a place at least, x r' and its rounding
+    change by less than 2^-42 |x r|), so these values decide for all others.  Exponents only shift it."""
+    s = Fraction(m, 8)
+    nearest = _to_24_bits(1 / s)
+    for places in range(-2, 3):
+        r = nearest + places * Fraction(2) ** (math.frexp(float(nearest))[1] - 24)
+        rest = _to_24_bits(_to_24_bits(1 - r * s) * r)
+        for border in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0):
+            b = Fraction(border)
+            for x, side in _neighbours(b * s):
+                q = _to_24_bits(x * r + _to_24_bits(x * rest))
+                assert (q > b) - (q < b) == side, (m, places, border, side)
+
+
+def test_sixth_of_two_operations_on_and_beside_the_borders():
+    """The same for the block scale of the NV form, largest / 6 as largest * RN(1 / 6) + largest * (what that rounding
+    left): on every border between E4M3 numbers and one last place beside it."""
+    sixth = _to_24_bits(Fraction(1, 6))
+    rest = _to_24_bits(Fraction(1, 6) - sixth)
+    for lo, hi in zip(ref.E4M3[0:126], ref.E4M3[1:127]):
+        b = (Fraction(lo) + Fraction(hi)) / 2
+        for x, side in _neighbours(6 * b):
+            q = _to_24_bits(x * sixth + _to_24_bits(x * rest))
+            assert (q > b) - (q < b) == side, (lo, side)

@@ -9,8 +9,9 @@
 //       bits) lies more than half of its last place away from it, and so does one by 6 from a border of
 //       E4M3 (5 bits): rounded to 24 bits it stays on its side, and on the border it stays there, if only
 //       the error before that rounding is small.  So the quotient is x r + x r', r an approximate reciprocal
-//       and r' = r (1 - r s) its Newton correction: two operations a value (checked for every 24-bit x,
-//       every s and border).
+//       and r' = r (1 - r s) its Newton correction: two operations a value.  It grows with x, so the
+//       borders and one last place beside them decide for every x: tests take all of them, under every s,
+//       in exact arithmetic for any r within two last places and on the device.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
