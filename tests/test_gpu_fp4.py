@@ -333,6 +333,65 @@ def test_many_rows_equal_their_slices(tb, torch_cuda, fmt):
     assert at == rows
 
 
+@pytest.mark.parametrize("rows,k,n", [(3, 100, 70), (2, 2000, 40), (40, 2048, 200), (300, 200, 150), (2000, 64, 96)])
+@pytest.mark.parametrize("ex,ew", [(100, 35), (30, 100), (-60, -70), (100, -100), (-100, 100)])
+def test_exponents_whose_sum_leaves_fp32(tb, torch_cuda, rows, k, n, ex, ew):
+    """2^(ex + ew) need not be an FP32 number: the results are those at exponents 0, shifted.  Beyond FP32's largest
+    number (sums of 2000 terms of 1e-4 have a deviation of 0.0045, times 2^135 2e38 of 3.4e38) they are infinite, below
+    its smallest normal one (all of (-60, -70)) they may be zero."""
+    torch = torch_cuda
+    x = activations(torch, rows, k, 91, spread=0.0) * 0.01
+    w = torch.randn(n, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(92)) * 0.01
+    shift = lambda t, e: (t.double() * 2.0 ** e).float()
+    f0 = tb.Fp4Filter(w, k, n, format=ref.NV, exponent=0)
+    f = tb.Fp4Filter(shift(w, ew), k, n, format=ref.NV, exponent=ew)
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    want, y = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, device="cuda")
+    tb.fp4_linear(f0, x, want, rows, work)
+    tb.fp4_linear(f, shift(x, ex), y, rows, work, ex)
+    want = (want.double() * 2.0 ** (ex + ew)).float()
+    assert bool(((y == want) | ((want.abs() < 2.0 ** -126) & (y == 0))).all())
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 2048, 1000), (3, 300, 140), (40, 2048, 200), (300, 512, 255), (2000, 64, 256)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_bias_and_relu_are_rounded_once(tb, torch_cuda, rows, k, n, dtype):
+    torch = torch_cuda
+    f, _ = filter_and_weights(tb, torch, n, k, ref.MX, 61)
+    x = activations(torch, rows, k, 62, spread=1.0)
+    bias = torch.randn(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(63))
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    plain, y = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, dtype=dtypes(torch)[dtype], device="cuda")
+    tb.fp4_linear(f, x, plain, rows, work)
+    tb.fp4_linear(f, x, y, rows, work, bias=bias)
+    assert torch.equal(y, (plain + bias).to(y.dtype))
+    tb.fp4_linear(f, x, y, rows, work, bias=bias, relu=True)
+    assert torch.equal(y, torch.relu(plain + bias).to(y.dtype))
+    tb.fp4_linear(f, x, y, rows, work, relu=True)
+    assert torch.equal(y, torch.relu(plain).to(y.dtype))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,k,n", [(1, (1 << 20) + 33, 40), (5, (1 << 20) - 1, 130), (300, 300001, 40), (2, 1 << 24, 9), (200, 1 << 18, 3000)])
+def test_long_sums_of_whole_numbers_are_exact(tb, torch_cuda, fmt, rows, k, n):
+    """Values 0, 1 and -1: every partial sum is a whole number below 2^24, whatever the order.  The NV form holds 1 as
+    6 E4M3(1 / 6) = 33/32: there a sum is 33^2 / 2^10 times a whole number, which stays below 2^24 / 33^2 = 15406 (sums
+    of 2^24 terms have a deviation of 2730)."""
+    torch = torch_cuda
+    g = torch.Generator(device="cuda").manual_seed(k)
+    signs = lambda r: torch.randint(-1, 2, (r, k), device="cuda", generator=g, dtype=torch.int8).to(torch.bfloat16)
+    x, w = signs(rows), signs(n)
+    f = tb.Fp4Filter(w, k, n, format=fmt, exponent=0)
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    y = torch.empty(rows, n, device="cuda")
+    tb.fp4_linear(f, x, y, rows, work)
+    f.check()
+    want = torch.zeros(rows, n, dtype=torch.float64, device="cuda")
+    for c in range(0, k, 1 << 18):
+        want += x[:, c:c + (1 << 18)].double() @ w[:, c:c + (1 << 18)].double().t()
+    assert torch.equal(y.double(), want * (1 if fmt == ref.MX else (33 / 32) ** 2))
+
+
 # ---- layers -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("n,h,w,ic,oc,stride", [(1, 1, 1, 8, 8, 1), (2, 7, 5, 64, 40, 1), (3, 9, 8, 33, 130, 2), (1, 14, 14, 256, 128, 2),
