@@ -333,12 +333,14 @@ int tetris_filter_file_check(const char *path, tetris_filter_info_t *info);
  *   TETRIS_FP4_MX  blocks of 32 columns; scale 2^e as a byte e + 127 (E8M0),
  *                  e = floor(log2(largest |x|)) - 2, at least -127; `exponent` has to be 0
  *   TETRIS_FP4_NV  blocks of 16 columns of u = x * 2^-exponent; scale = (largest |u|) / 6 rounded
- *                  to E4M3 (at most 448).  2688 * 2^exponent is the largest value that can be held,
+ *                  to E4M3 (at most 448).  2688 * 2^exponent is the largest value that can be held (larger
+ *                  ones become it, without a sign to the caller),
  *                  blocks whose largest value is at most 6 * 2^(exponent - 10) become zero.
  *                  The tensor's own scale is a power of two so that every border between two codes
  *                  is an exact FP32 number: quantisation is exact, not off by a rounding now and then.
- * A code is x (u) over its block's scale, rounded to nearest, ties to the even code, at most 6.  A block with an infinity or a NaN takes the scale NaN (0xFF; 0x7F) and reads back
- * as NaN, as does every product through it.  -100 <= exponent <= 100.
+ * A code is x (u) over its block's scale, rounded to nearest, ties to the even code, at most 6.  A block with an
+ * infinity or a NaN takes the scale NaN (0xFF; 0x7F) and reads back as NaN, as does every product
+ * through it.  -100 <= exponent <= 100.
  * Sums run in FP32; results below FP32's normal numbers may become zero.
  *
  * Storage of a matrix of `rows` x `cols`, the columns being what a product sums over:
@@ -353,7 +355,8 @@ int tetris_filter_file_check(const char *path, tetris_filter_info_t *info);
  * Types of activations, results and dense weights: TETRIS_FP32, TETRIS_BF16, TETRIS_FP16; `ld` is the
  * distance between rows in elements (0: rows lie close).  Tensors need the alignment of their type only;
  * 16-byte aligned rows take the vector paths.  An output must not overlap an input.
- * The calls are asynchronous on `stream`, allocate nothing and keep nothing between calls; the device
+ * The calls are asynchronous on `stream` and allocate nothing.  A filter keeps the tile geometry of the
+ * last few numbers of rows that it was multiplied with; nothing else is kept between calls.  The device
  * of the filter is made current for the call, the calls without a filter run on the current device.
  * Results are bit-reproducible from call to call.
  */

@@ -555,7 +555,7 @@ class Fp4Filter:
     """The weights of a 1x1 (or fully connected) layer in 4 bits, living on one GPU.
 
     Beside SparseFilter: dense [out_channel][in_channel] `filter` (numpy array, or a tensor on the host
-    or on `device`), quantised on the device.  `exponent` is the whole filter's in the FP4_NV format
+    or on `device`, there complete in the order of `cuda_stream`), quantised on the device.  `exponent` is the whole filter's in the FP4_NV format
     (FP4_EXPONENT_AUTO: the smallest that holds the largest weight).  It owns device memory, freed by
     close() or garbage collection.
     """

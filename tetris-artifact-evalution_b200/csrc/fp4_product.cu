@@ -3,10 +3,13 @@
 // tcgen05.mma with block scales: kind::mxf4 (32 values a scale, E8M0) and kind::mxf4nvf4 (16 a scale,
 // E4M3), both 64 values of K per instruction, FP32 accumulators in tensor memory.
 //
-// What bounds it: large products the tensor cores and the card's power (4096x4096x16384, MX: 3.8 to 4.2 PFLOP/s at
-// 1.6 to 1.9 GHz and 1000 W; the MMAs alone, without loads and copies of scales, 5.5); few rows the reading of the
-// filter (16x8192x8192, NV: 9.4 us, 4.1 TB/s); layers with few columns the writing of the output (50176x64x256: 11.1 us,
-// 4.8 TB/s); small products the launch (1x2048x1000: 3 us).
+// What bounds it.  Large products: clocks of an SM, 230 to 260 for each MMA of N = 256 that could take 128, at any clock
+// rate (205 without loads and copies of scales: operands from shared memory), and 1.1 to 1.6 us from tile to tile.  The
+// clock falls as the card reaches 1000 W: 4096x4096x16384 MX takes 131 us at 1.95 GHz (the first 300 calls after a
+// pause, 4.2 PFLOP/s) and 151 at 1.55 to 1.6 GHz (6000 calls in a row, 3.65 PFLOP/s), 8192x4096x8192 NV 136 and 157.
+// Few rows: 2 us of launch, first loads and cluster meeting, then the filter at 5.2 TB/s (1x4096x4096 MX 3.7 us,
+// 16x8192x8192 NV 9.3).  Hundreds of rows: the K steps one after the other, 0.36 us each, and 3 us beside them
+// (333x2048x1000 NV 6.0 us).  Layers with few columns: the writing of the output (50176x64x256: 11.1 us, 4.8 TB/s).
 //
 // Which operand is on the M side (128 lanes of tensor memory) depends on the number of rows.
 //   Few rows: the filter, D[oc][row].  16 to 64 rows cost a narrow N instead of an empty M; a lane is a channel,
@@ -724,9 +727,9 @@ constexpr size_t kSmemMost = 227 * 1024, kSmemHalf = 113 * 1024;   // (1 KB of e
 constexpr size_t kSmemLeast = 117 * 1024;
 
 // A product quantises its rows itself where a storing warp has at most this many units of it to do.  Up to there it takes
-// no longer than a launch of its own before the product, and the host has one launch less, 2.2 us (16x1024x1024, 2 units:
-// 4.1 us on the device in one launch, 4.5 in two; 22x832x32, 4 units: 5.2 and 4.5; 51x1824x640, 8 units: 7.5 and 5.8;
-// 16x8192x8192, 16 units: 18 and 10.7).
+// about as long as a launch of its own before the product (16x1024x1024, 2 units: 4.1 us on the device in one launch,
+// 4.3 in two; 22x832x32, 4 units: 4.8 and 4.5; 51x1824x640, 8 units: 7.5 and 5.8; 16x8192x8192, 16 units: 18 and 10.8),
+// and the host has one launch less, 2.2 us.  At four units the host is why: a captured graph pays 0.3 us for it.
 constexpr int kDirectUnits = 4;
 
 // How the rows of a tile are cut into units of a warp: 2^lx lanes take a row's part of a K step.
@@ -751,7 +754,9 @@ struct Geometry {
 int row_log_of(int cols) { return cols <= 64 ? 5 : cols <= 128 ? 6 : 7; }
 
 // The least of an estimate in nanoseconds, whose terms were fitted to 60 shapes (1 to 50000 rows, 64 to 16384
-// columns and channels) in every geometry: its choice takes 1.5 % longer than the best, 15 % at worst.
+// columns and channels, columns in multiples of 64 and channels in multiples of 16) in every geometry: its choice takes
+// 1.5 % longer than the best of those, 15 % at worst.  It has no term for outputs that TMA stores do not take
+// (1352x1024 to 255 channels 4.8 us, to 256 4.2).
 //   a K step    the longer of its MMAs and its loads: 51 bytes a nanosecond for half an SM alone, 2 x 40 for two
 //               halves, 75 for a whole one (16x8192x8192: 12.2 us in 128 halves, 9.5 in 256)
 //   a tile      the longer of its steps and the store of the one before it; the last store stands alone
