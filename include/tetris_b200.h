@@ -402,7 +402,7 @@ int tetris_fp4_filter_check(const tetris_fp4_filter_t *f);
  *   tetris_fp4_conv2d   the 1x1 layer: FP32 NHWC in and out as tetris_conv2d_launch, padding must be 0
  * `d_workspace` holds the quantised activations: tetris_fp4_workspace(f, rows) bytes (rows = N * OH * OW
  * for the layer), 16-byte aligned.  0 bytes (NULL) where so few rows are quantised by the product itself, in one
- * launch.  It is free again when the call has passed on its stream; calls that can run at the same time (other
+ * launch.  What is enough for some rows is enough for fewer.  It is free again when the call has passed on its stream; calls that can run at the same time (other
  * streams, graphs that are replayed side by side) each need their own.
  */
 int tetris_fp4_product(const tetris_fp4_filter_t *f, const void *d_codes, const void *d_scales, int64_t rows, int exponent,

@@ -392,6 +392,27 @@ def test_long_sums_of_whole_numbers_are_exact(tb, torch_cuda, fmt, rows, k, n):
     assert torch.equal(y.double(), want * (1 if fmt == ref.MX else (33 / 32) ** 2))
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("k,n", [(100, 2048), (128, 512), (64, 16), (300, 300), (2048, 1000)])
+def test_a_workspace_for_some_rows_is_enough_for_fewer(tb, torch_cuda, fmt, k, n):
+    """A program that serves changing numbers of rows takes one workspace, for the most."""
+    torch = torch_cuda
+    f, w = filter_and_weights(tb, torch, n, k, fmt, 41)
+    most = 2500
+    sizes = [tb.fp4_workspace(f, r) for r in range(1, most + 1)]
+    assert sizes == sorted(sizes)
+    x = activations(torch, most, k, 42, spread=1.0)
+    want, terms = reference_product(x, w, fmt, 0, f.exponent_)
+    for rows in (513, 1793, 2305, 2500):
+        work = torch.empty(sizes[rows - 1], dtype=torch.uint8, device="cuda")
+        for fewer in (1, 17, 509, 1789, 2301):
+            if fewer <= rows:
+                y = torch.empty(fewer, n, device="cuda")
+                tb.fp4_linear(f, x[:fewer], y, fewer, work)
+                check_product(y, want[:fewer], terms[:fewer], k, torch)
+    f.check()
+
+
 # ---- layers -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("n,h,w,ic,oc,stride", [(1, 1, 1, 8, 8, 1), (2, 7, 5, 64, 40, 1), (3, 9, 8, 33, 130, 2), (1, 14, 14, 256, 128, 2),

@@ -632,7 +632,7 @@ def fp4_product(fp4_filter, codes, scales, output, rows, exponent=0, bias=None, 
 
 
 def fp4_workspace(fp4_filter, rows):
-    """Bytes of device workspace that fp4_linear and fp4_conv2d need for `rows` rows (pixels)."""
+    """Bytes of device workspace that fp4_linear and fp4_conv2d need for `rows` rows (pixels) or fewer."""
     _fp4_longs(rows)
     n = ctypes.c_int64(0)
     _check(lib().tetris_fp4_workspace(fp4_filter.handle, rows, ctypes.byref(n)))

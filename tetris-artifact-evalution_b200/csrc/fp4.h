@@ -13,6 +13,7 @@ struct tetris_fp4_filter {
   int format, exponent;
   int device, sm_count;
   int64_t pitch, code_bytes, scale_bytes;
+  int64_t direct_rows;     // a product of up to so many rows quantises them itself
   uint8_t *d_codes, *d_scales;
   int *d_error;            // raised by a product that gave up on a barrier wait
   // geometries of the last numbers of rows (fp4_product.cu): the number in the upper 40 bits, 0: none yet
@@ -68,9 +69,9 @@ struct Fp4Rows {             // activations of a product
   int64_t ld;
   const Fp4Pixels *px;
 };
-// whether a product of so many rows quantises them itself (else they are quantised into a workspace first); its sums
-// are the same either way
-bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows);
+// The rows up to which a product quantises them itself (more are quantised into a workspace first; the sums are the same
+// either way): one number, so that a workspace for some rows is enough for fewer.
+int64_t fp4_product_direct_rows(const tetris_fp4_filter *f);
 int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
                        int relu, cudaStream_t st);
 

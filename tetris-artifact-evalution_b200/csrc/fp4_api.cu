@@ -62,7 +62,7 @@ int check_filter(const tetris_fp4_filter *f) {
 
 int64_t workspace_codes(const tetris_fp4_filter *f, int64_t rows) { return (rows * f->pitch + 255) / 256 * 256; }
 int64_t workspace_bytes(const tetris_fp4_filter *f, int64_t rows) {
-  return rows == 0 || fp4_product_direct(f, rows) ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
+  return rows <= f->direct_rows ? 0 : workspace_codes(f, rows) + fp4_scale_bytes(rows, f->in_channel, f->format);
 }
 
 // Checks that all products share; the filter's device is current.
@@ -190,6 +190,7 @@ int tetris_fp4_filter_create(const void *weights, int w_type, int in_channel, in
     set_error("device attributes: %s", cudaGetErrorString(cudaGetLastError()));
     return fail(TETRIS_ERR_CUDA);
   }
+  f->direct_rows = fp4_product_direct_rows(f);
   if (!alloc((void **)&f->d_codes, f->code_bytes, "the codes") || !alloc((void **)&f->d_scales, f->scale_bytes, "the scales") ||
       !alloc((void **)&f->d_error, sizeof(int), "the error flag") || !alloc((void **)&d_bits, sizeof(unsigned), "the largest weight") ||
       (!on_device && !alloc(&d_dense, dense_bytes, "the dense filter")))

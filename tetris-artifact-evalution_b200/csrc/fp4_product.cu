@@ -746,7 +746,6 @@ struct Geometry {
   bool rows_m;
   int nt, d;
   bool half;
-  bool direct;             // rows that come as they are: quantised by the product
 };
 
 // Bytes of a row's codes in a stage, as a logarithm: a TMA load takes its time for the zeros behind the last column, too
@@ -768,7 +767,7 @@ int row_log_of(int cols) { return cols <= 64 ? 5 : cols <= 128 ? 6 : 7; }
 Geometry estimate(const tetris_fp4_filter *f, int64_t rows) {
   const int steps = (f->in_channel + kStep - 1) / kStep;
   const double sms = f->sm_count, row_bytes = (1 << row_log_of(f->in_channel)) + (f->format == TETRIS_FP4_NV ? 16 : 8);  // of a step
-  Geometry best = {false, 16, 1, true, false};
+  Geometry best = {false, 16, 1, true};
   double least = 1e300;
   for (int rows_m = 0; rows_m < 2; ++rows_m) {
     const int64_t m = rows_m ? rows : f->out_channel, n = rows_m ? f->out_channel : rows;
@@ -793,7 +792,7 @@ Geometry estimate(const tetris_fp4_filter *f, int64_t rows) {
             cost = rounds * std::max(k * std::max(bytes / 75., 1.1 * nt), store) + (rounds - 1) * (nt > 128 ? 500. : 580.) + 36. + (2 * ctas > sms ? 620. : 0.);
           }
           cost += d > 1 ? 100. + 20. * nt : store;
-          if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0, false}; }
+          if (cost < least) { least = cost; best = {rows_m != 0, nt, d, half != 0}; }
         }
       }
     }
@@ -813,12 +812,11 @@ bool is_direct(const tetris_fp4_filter *f, int64_t rows, const Geometry &g) {
 Geometry choose(const tetris_fp4_filter *f, int64_t rows) {
   std::atomic<uint64_t> &kept = f->plans[rows & 7];
   const uint64_t k = kept.load(std::memory_order_relaxed);
-  if (k >> 24 == (uint64_t)rows) return {(k & 1) != 0, (int)(k >> 8 & 0x1FF), 1 << (k >> 4 & 3), (k & 2) != 0, (k & 4) != 0};
-  Geometry g = estimate(f, rows);
-  g.direct = is_direct(f, rows, g);
+  if (k >> 24 == (uint64_t)rows) return {(k & 1) != 0, (int)(k >> 8 & 0x1FF), 1 << (k >> 4 & 3), (k & 2) != 0};
+  const Geometry g = estimate(f, rows);
   int d_log = 0;
   while (1 << d_log < g.d) ++d_log;
-  kept.store((uint64_t)rows << 24 | (uint64_t)g.nt << 8 | (uint64_t)d_log << 4 | (g.direct ? 4 : 0) | (g.half ? 2 : 0) | (g.rows_m ? 1 : 0), std::memory_order_relaxed);
+  kept.store((uint64_t)rows << 24 | (uint64_t)g.nt << 8 | (uint64_t)d_log << 4 | (g.half ? 2 : 0) | (g.rows_m ? 1 : 0), std::memory_order_relaxed);
   return g;
 }
 
@@ -857,7 +855,12 @@ int encode(CUtensorMap *map, CUtensorMapDataType type, int type_bytes, const voi
 
 }  // namespace
 
-bool fp4_product_direct(const tetris_fp4_filter *f, int64_t rows) { return choose(f, rows).direct; }
+// Geometries and units change behind powers of two and multiples of 16 rows.
+int64_t fp4_product_direct_rows(const tetris_fp4_filter *f) {
+  int64_t rows = 0;
+  for (int64_t next = 1; is_direct(f, next, estimate(f, next)); next += next < 16 ? next : 16) rows = next;
+  return rows;
+}
 
 int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t rows, int exponent, const float *bias, void *y, int y_type, int64_t ld,
                        int relu, cudaStream_t st) {
