@@ -277,6 +277,30 @@ def test_rows_apart_in_and_out(tb, torch_cuda, fmt, rows):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,n,ld", [(19, 1, 2, 8), (5, 64, 7, 16), (300, 64, 30, 40), (300, 64, 27, 32), (700, 300, 130, 136), (2000, 512, 250, 264),
+                                         (2000, 512, 255, 256), (3000, 256, 513, 520)])
+def test_aligned_rows_apart_whose_ends_are_not(tb, torch_cuda, fmt, dtype, rows, k, n, ld):
+    """Rows of an output that begin on 16 bytes and end inside of them: what lies between the rows, and behind the last
+    one of a buffer that ends with it, stays as it was."""
+    torch = torch_cuda
+    f, w = filter_and_weights(tb, torch, n, k, fmt, 51)
+    x = activations(torch, rows, k, 52, spread=1.0)
+    work = torch.empty(tb.fp4_workspace(f, rows), dtype=torch.uint8, device="cuda")
+    want = torch.empty(rows, n, device="cuda")
+    tb.fp4_linear(f, x, want, rows, work)
+    check_product(want, *reference_product(x, w, fmt, 0, f.exponent_), k, torch)
+    need = (rows - 1) * ld + n
+    whole = torch.full((need + 64,), -3.0, dtype=dtypes(torch)[dtype], device="cuda")
+    tb.fp4_linear(f, x, whole[:need], rows, work, ld_output=ld)
+    f.check()
+    assert bool((whole[need:] == -3.0).all())
+    out = torch.cat([whole[:need], whole[need:need + ld - n]]).view(rows, ld)
+    assert torch.equal(out[:, :n], want.to(out.dtype))
+    assert bool((out[:, n:] == -3.0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows", [3, 40, 300])
 def test_nan_stays_in_its_row_and_channel(tb, torch_cuda, fmt, rows):
     torch = torch_cuda

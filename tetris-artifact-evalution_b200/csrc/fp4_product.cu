@@ -92,7 +92,7 @@ struct ProductParams {
   int lx, unit_log;        // log2 of the lanes of a row, of the units (32 lanes) of a tile's rows in a K step
   float tensor_scale, sixth, sixth_rest;  // as in the quantisation
   int relu;
-  int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows)
+  int tma_store;           // D[row][oc]: the output takes TMA stores (16-byte aligned rows of whole 16 bytes)
   int staging;             // ... staging blocks of a storing warp: 1 or 2
   int *error_flag;
   unsigned spin_limit;
@@ -919,8 +919,11 @@ int launch_fp4_product(const tetris_fp4_filter *f, const Fp4Rows &a, int64_t row
     fp4_scale_factors(exponent, &p.tensor_scale, &p.sixth, &p.sixth_rest);
   }
   p.relu = relu;
-  // (the distance between rows in a tensor map is below 2^40 bytes)
-  p.tma_store = g.rows_m && g.d == 1 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes)) & 15) == 0 && ld * bytes < (1ll << 40);
+  // A TMA store leaves out what lies behind a row's end by whole 16 bytes only: a row that ends inside of them would have
+  // zeros written behind it, into whatever lies between rows that are apart.  (The distance between rows in a tensor
+  // map is below 2^40 bytes.)
+  p.tma_store = g.rows_m && g.d == 1 && ((reinterpret_cast<uintptr_t>(y) | (uint64_t)(ld * bytes) | (uint64_t)f->out_channel * bytes) & 15) == 0 &&
+                ld * bytes < (1ll << 40);
   p.error_flag = f->d_error;
   p.withhold_first_load = test_injection(&p.spin_limit);
   CUtensorMap map_w, map_a = {}, map_y = {};
